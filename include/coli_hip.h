@@ -305,6 +305,110 @@ int   coli_hip_gemm_tile(const ColiVkTensor *t, int S, int *parts);
  * counterpart in the reference. */
 int   coli_hip_gdn_chunked(int on);
 
+/* ---- paged key-value cache of many sequences ----
+ * One pool of fixed-size pages holds the keys and values of every sequence and layer:
+ *   data  [n_pages][n_layers][2 (K, V)][KH][page][hd] of `dtype`, aligned to 16 bytes
+ *   table [n_seqs][max_pages] page ids; the first ceil(len / page) of a row are in use, the
+ *         others are -1
+ *   lens  [n_seqs] positions held
+ *   refs  [n_pages] table entries that hold the page (0: free)
+ *   used  [ceil(n_pages / 32)] bitmap of pages in use (bit p % 32 of word p / 32)
+ *   state [COLI_HIP_PAGES_STATE] error bits and words of the library
+ *   work  [coli_hip_pages_work()] ints of scratch, no contents kept between calls
+ * All arrays are the caller's device memory; coli_hip_pages_init fills the bookkeeping ones
+ * (not data).  hd is a multiple of 8 in 8..256, page 1..4096.
+ * The functions read and change the arrays on the device, in stream order, with no host
+ * decision: a decode step (append, then per layer qk_rope and attn) can be captured into a
+ * graph.  Calls on one pool that change it (init, append, fork, free, compact, qk_rope) must be
+ * ordered: one stream, or events between streams.  In every list of sequences -1 stands for
+ * "none" (padding of a fixed-size batch).  What only the device can see is not reported by the
+ * return value but gathered in the pool's error bits (coli_hip_pages_status). */
+enum { COLI_HIP_F32 = 0, COLI_HIP_F16 = 1, COLI_HIP_BF16 = 2 };
+enum { COLI_HIP_PAGES_STATE = 16 };
+typedef struct {
+    void *data;
+    int *table, *lens, *refs;
+    unsigned *used;
+    int *state, *work;
+    int dtype, n_layers, KH, hd, page, n_pages, n_seqs, max_pages;
+} ColiHipPages;
+/* 1 when the description is one the library takes (host only, no device needed), else 0 with a
+ * message.  Every function below checks it as well. */
+int    coli_hip_pages_check(const ColiHipPages *p);
+/* ints that `work` has to hold. */
+size_t coli_hip_pages_work(const ColiHipPages *p);
+/* An empty pool: every page free, every sequence of length 0. */
+int    coli_hip_pages_init(const ColiHipPages *p, void *stream);
+/* Sequence d_seq[i] grows by d_count[i] >= 0 positions (d_count NULL: 1), n <= 4096.  New pages
+ * are taken lowest free page first, in the order of the list; the new positions' K and V are
+ * whatever the pages hold until qk_rope writes them.  All or nothing: when pages or a table row
+ * do not suffice, or a sequence is named twice, nothing changes and an error bit is set. */
+int    coli_hip_pages_append(const ColiHipPages *p, const int *d_seq, const int *d_count, int n, void *stream);
+/* Sequence d_dst[i], which must be empty, becomes a copy of d_src[i] (a pair with a -1 is
+ * skipped), n <= 4096.  share != 0: full pages are shared (their counts grow), the last, partly
+ * filled page is copied, so a position appended later lands in a page of its own sequence;
+ * share == 0: every page is copied.  Only positions held are copied.  All or nothing as above.
+ * Overwriting an earlier position of a shared page (qk_rope with d_pos) is seen by all its
+ * sequences. */
+int    coli_hip_pages_fork(const ColiHipPages *p, const int *d_src, const int *d_dst, int n, int share, void *stream);
+/* Sequences d_seq[i] end, n <= 4096: their lengths become 0, pages no other sequence holds are
+ * free.  An empty sequence, or one named twice, is freed once. */
+int    coli_hip_pages_free(const ColiHipPages *p, const int *d_seq, int n, void *stream);
+/* The pool closed up: with L pages in use, the used pages at or past L move, in order, into the
+ * free pages below L, and the tables follow.  Pages [L, n_pages) are free afterwards. */
+int    coli_hip_pages_compact(const ColiHipPages *p, void *stream);
+/* Waits for the stream; the number of free pages and the error bits gathered since the last
+ * call (cleared by it): 1 not enough free pages, 2 a sequence longer than its table row, 4 a
+ * sequence, count or position out of range, 8 a sequence twice in a call or a fork into one
+ * that is not empty, 16 a position past its sequence's end, 32 a table entry that is no page.
+ * Either pointer may be NULL.  Refused while the stream is being captured. */
+int    coli_hip_pages_status(const ColiHipPages *p, int *n_free, int *errors, void *stream);
+
+/* The heads of an attention layer over a pool (what a program keeps per layer).  Strides are in
+ * floats: query head h of row r is at q + r * q_row + h * q_head (with the gate beside it where
+ * the projection is gated: q_head = 2 hd, gate = q + hd); key head h at k + r * kv_row + h * hd,
+ * the values alike. */
+typedef struct {
+    int H;                    /* query heads, a multiple of KH */
+    int rot;                  /* rotary columns, even, 0..hd */
+    int interleaved;          /* pairs (2j, 2j + 1); 0: (j, j + rot / 2) */
+    int64_t q_row, q_head, kv_row;
+    float eps;                /* of the norms */
+    float rope_mag;           /* factor of the rotated columns (1 where contexts are not scaled) */
+    float scale;              /* of the scores, usually 1 / sqrt(hd) */
+    const float *qn, *kn;     /* zero-centred norm weights [hd], device; NULL: no norm */
+    const float *freq;        /* inverse frequencies [rot / 2], device (any scaling of contexts is in them) */
+} ColiHipHeads;
+int    coli_hip_heads_check(const ColiHipPages *p, const ColiHipHeads *h);
+/* Rows i < n of q, k and v of sequence d_seq[i] at position d_pos[i] (d_pos NULL: the last one,
+ * lens - 1): queries normed and rotated into d_qout [n][H][hd], keys normed, rotated and rounded
+ * into the sequence's page of the layer, values rounded beside them.  The position must be held
+ * already (append first): a row past the end, or with sequence -1, is skipped whole.  Two rows
+ * with one position leave either's K and V.  Angles are pos * freq in 64 bits. */
+int    coli_hip_qk_rope_paged(const ColiHipPages *p, const ColiHipHeads *h, int layer, const float *d_q,
+                              const float *d_k, const float *d_v, const int *d_seq, const int *d_pos, int n,
+                              float *d_qout, void *stream);
+/* Attention of row i over positions 0..d_pos[i] of sequence d_seq[i] (d_pos NULL: all of it):
+ * d_out [n][H][hd] = softmax(scale q k^T) v, times sigmoid(gate) where d_gate is not NULL
+ * (strides q_row, q_head).  d_q is [n][H][hd] as qk_rope leaves it.  A row that sees no position
+ * gives 0; a row with sequence -1 is left as it was; one past the end sees what the sequence
+ * holds.  max_len: the longest sequence in the call as far as the caller knows (0: unknown); only the split
+ * of the work goes by it.  d_work: coli_hip_attn_paged_work() bytes, aligned to 16, zeroed once
+ * before its first use and not shared by calls that may run at once. */
+size_t coli_hip_attn_paged_work(const ColiHipPages *p, const ColiHipHeads *h);
+int    coli_hip_attn_paged(const ColiHipPages *p, const ColiHipHeads *h, int layer, const float *d_q,
+                           const float *d_gate, const int *d_seq, const int *d_pos, int n, int max_len, float *d_out,
+                           void *d_work, size_t work_bytes, void *stream);
+/* An attention layer of n rows of many sequences, the batch form of coli_vk_gqa_full on device
+ * rows: d_x [n][D] (normed) -> q (| gate where gq_t has 2 H hd rows), k, v -> qk_rope into the
+ * pages -> attention -> out_t -> d_out [n][out_t rows].  The positions must have been appended.
+ * A row with sequence -1 gives 0.  The strides of h are not used.  Shares the layer blocks'
+ * scratch: one stream. */
+int    coli_hip_gqa_paged(const ColiHipPages *p, const ColiHipHeads *h, int layer, const float *d_x, int D,
+                          const ColiVkTensor *gq_t, const ColiVkTensor *gk_t, const ColiVkTensor *gv_t,
+                          const ColiVkTensor *out_t, const int *d_seq, const int *d_pos, int n, int max_len,
+                          float *d_out, void *stream);
+
 /* ---- fmt=6 container reader (c/st.h:120-456, c/qwen.c:509-536) ----
  * The safetensors shards c/tools/convert_qwen35_moe.py writes (U8 int4 nibbles plus an F32
  * ".qs" tensor of [scale, zero] pairs per group) read straight into device tensors.

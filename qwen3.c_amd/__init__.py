@@ -111,6 +111,19 @@ _SIGS = {
     "coli_vk_stream_moe_fused": (_I, []),
     "coli_vk_stream_ix_pending": (_I, []),
     "coli_vk_stream_ix_hist": (_I, [_I, _P, _I]),
+    "coli_hip_pages_check": (_I, [_P]),
+    "coli_hip_pages_work": (C.c_size_t, [_P]),
+    "coli_hip_pages_init": (_I, [_P, _P]),
+    "coli_hip_pages_append": (_I, [_P, _P, _P, _I, _P]),
+    "coli_hip_pages_fork": (_I, [_P, _P, _P, _I, _I, _P]),
+    "coli_hip_pages_free": (_I, [_P, _P, _I, _P]),
+    "coli_hip_pages_compact": (_I, [_P, _P]),
+    "coli_hip_pages_status": (_I, [_P, _P, _P, _P]),
+    "coli_hip_heads_check": (_I, [_P, _P]),
+    "coli_hip_qk_rope_paged": (_I, [_P, _P, _I, _P, _P, _P, _P, _P, _I, _P, _P]),
+    "coli_hip_attn_paged_work": (C.c_size_t, [_P, _P]),
+    "coli_hip_attn_paged": (_I, [_P, _P, _I, _P, _P, _P, _P, _I, _I, _P, _P, C.c_size_t, _P]),
+    "coli_hip_gqa_paged": (_I, [_P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P]),
 }
 
 
@@ -140,6 +153,21 @@ class Tensor:
 
     def nbytes(self):
         return int(self.lib.L.coli_vk_tensor_bytes(self.handle))
+
+
+class Pages(C.Structure):
+    """ColiHipPages: a pool of key-value pages in the caller's device memory."""
+
+    _fields_ = [(n, _P) for n in ("data", "table", "lens", "refs", "used", "state", "work")] + [
+        (n, _I) for n in ("dtype", "n_layers", "KH", "hd", "page", "n_pages", "n_seqs", "max_pages")]
+
+
+class Heads(C.Structure):
+    """ColiHipHeads: an attention layer's heads over a pool."""
+
+    _fields_ = [("H", _I), ("rot", _I), ("interleaved", _I), ("q_row", C.c_int64), ("q_head", C.c_int64),
+                ("kv_row", C.c_int64), ("eps", _F), ("rope_mag", _F), ("scale", _F), ("qn", _P), ("kn", _P),
+                ("freq", _P)]
 
 
 class Container:
@@ -465,6 +493,64 @@ class Lib:
         a = np.ascontiguousarray(in_ln, dtype=np.float32)
         b = np.ascontiguousarray(post_ln, dtype=np.float32)
         self._ok(self.L.coli_vk_layer_norm_weight(layer, _ptr(a), _ptr(b), a.size), "coli_vk_layer_norm_weight")
+
+    # ---- paged key-value cache ----------------------------------------------------
+    F32, F16, BF16 = 0, 1, 2   # page types
+    PAGES_STATE = 16           # ints of a pool's state array
+
+    @staticmethod
+    def pages(data, table, lens, refs, used, state, work, dtype, n_layers, KH, hd, page, n_pages, n_seqs, max_pages):
+        """A pool over device addresses; keep what they belong to."""
+        return Pages(data, table, lens, refs, used, state, work, dtype, n_layers, KH, hd, page, n_pages, n_seqs,
+                     max_pages)
+
+    @staticmethod
+    def heads(H, rot, interleaved, q_row, q_head, kv_row, eps, rope_mag, scale, qn=None, kn=None, freq=None):
+        return Heads(H, rot, int(interleaved), q_row, q_head, kv_row, eps, rope_mag, scale, qn, kn, freq)
+
+    def pages_work(self, n_seqs, n_pages):
+        """ints of a pool's work array."""
+        return int(self.L.coli_hip_pages_work(C.byref(Pages(n_seqs=n_seqs, n_pages=n_pages))))
+
+    def pages_init(self, pool, stream=None):
+        self._ok(self.L.coli_hip_pages_init(C.byref(pool), stream), "coli_hip_pages_init")
+
+    def pages_append(self, pool, d_seq, d_count, n, stream=None):
+        self._ok(self.L.coli_hip_pages_append(C.byref(pool), d_seq, d_count, n, stream), "coli_hip_pages_append")
+
+    def pages_fork(self, pool, d_src, d_dst, n, share=True, stream=None):
+        self._ok(self.L.coli_hip_pages_fork(C.byref(pool), d_src, d_dst, n, int(share), stream), "coli_hip_pages_fork")
+
+    def pages_free(self, pool, d_seq, n, stream=None):
+        self._ok(self.L.coli_hip_pages_free(C.byref(pool), d_seq, n, stream), "coli_hip_pages_free")
+
+    def pages_compact(self, pool, stream=None):
+        self._ok(self.L.coli_hip_pages_compact(C.byref(pool), stream), "coli_hip_pages_compact")
+
+    def pages_status(self, pool, stream=None):
+        """(free pages, error bits since the last call); waits for the stream."""
+        fr, err = _I(0), _I(0)
+        self._ok(self.L.coli_hip_pages_status(C.byref(pool), C.byref(fr), C.byref(err), stream),
+                 "coli_hip_pages_status")
+        return fr.value, err.value
+
+    def qk_rope_paged_dev(self, pool, heads, layer, d_q, d_k, d_v, d_seq, d_pos, n, d_qout, stream=None):
+        self._ok(self.L.coli_hip_qk_rope_paged(C.byref(pool), C.byref(heads), layer, d_q, d_k, d_v, d_seq, d_pos, n,
+                                               d_qout, stream), "coli_hip_qk_rope_paged")
+
+    def attn_paged_work(self, pool, heads):
+        """Bytes of the attention's workspace."""
+        return int(self.L.coli_hip_attn_paged_work(C.byref(pool), C.byref(heads)))
+
+    def attn_paged_dev(self, pool, heads, layer, d_q, d_gate, d_seq, d_pos, n, max_len, d_out, d_work, work_bytes,
+                       stream=None):
+        self._ok(self.L.coli_hip_attn_paged(C.byref(pool), C.byref(heads), layer, d_q, d_gate, d_seq, d_pos, n,
+                                            max_len, d_out, d_work, work_bytes, stream), "coli_hip_attn_paged")
+
+    def gqa_paged_dev(self, pool, heads, layer, d_x, tq, tk, tv, to, d_seq, d_pos, n, max_len, d_out, stream=None):
+        self._ok(self.L.coli_hip_gqa_paged(C.byref(pool), C.byref(heads), layer, d_x, tq.I, tq.handle, tk.handle,
+                                           tv.handle, to.handle, d_seq, d_pos, n, max_len, d_out, stream),
+                 "coli_hip_gqa_paged")
 
     # ---- layer blocks on host rows ---------------------------------------------------
     def gqa_full(self, layer, x, tq, tk, tv, to, S, H, KH, hd, rot, pos_base, max_t, eps, theta):

@@ -166,6 +166,7 @@ void moe_shutdown();
 void prefill_shutdown();
 void layer_shutdown();
 void container_shutdown();
+void paged_shutdown();
 void scratch_free(void **p, size_t *cap);
 void host_scratch_free(void **p, size_t *cap);
 

@@ -1,0 +1,500 @@
+// pages.hip - the pages of a key-value cache that serves many sequences: taking pages for new
+// positions, forking and freeing sequences, closing up the pool.  No counterpart in the
+// reference, whose cache is one dense row per position of one sequence.
+//
+// Everything a decode loop changes lives on the device (tables, lengths, reference counts, the
+// bitmap of pages in use), so a step needs no host decision and can be captured.  Nothing
+// depends on the order of atomics: pages are taken lowest free one first in the order of the
+// call, counts are integers, and a page's bit falls with the count that reaches 0.  A page that
+// is not full belongs to one sequence alone (fork copies it), so a new position never lands in
+// a shared page.
+#include "paged.h"
+
+#include <stdio.h>
+#include <stdlib.h>
+
+namespace coli {
+
+constexpr int kPgThreads = 1024;     // the bookkeeping block
+constexpr int kPgMaxN = 4096;        // sequences of one call (their offsets are held in LDS)
+constexpr int kCopyThreads = 256;
+constexpr long kCopyPiece = 16384;   // bytes of a page that one block copies at a time
+
+bool paged_refuse(const char *why) {
+    fprintf(stderr, "[HIP] paged cache call refused: %s\n", why);
+    return false;
+}
+
+bool pool_view(const ColiHipPages *p, PoolView &v) {
+    if (!p || !p->data || !p->table || !p->lens || !p->refs || !p->used || !p->state || !p->work)
+        return paged_refuse("a pool pointer is NULL");
+    if (p->dtype != COLI_HIP_F32 && p->dtype != COLI_HIP_F16 && p->dtype != COLI_HIP_BF16)
+        return paged_refuse("page type");
+    if (p->hd < 8 || p->hd > 256 || p->hd % 8) return paged_refuse("head dim not a multiple of 8 in 8..256");
+    if (p->page < 1 || p->page > 4096) return paged_refuse("page size not in 1..4096");
+    if (p->KH < 1 || p->KH > 1024 || p->n_layers < 1 || p->n_layers > 4096) return paged_refuse("heads or layers");
+    if (p->n_pages < 1 || p->n_seqs < 1 || p->max_pages < 1) return paged_refuse("empty pool");
+    if ((long)p->max_pages * p->page >= 1L << 31 || p->n_pages > 1 << 30) return paged_refuse("pool too large");
+    if ((uintptr_t)p->data % 16) return paged_refuse("pool data not aligned to 16 bytes");
+    v.data = (char *)p->data;
+    v.table = p->table, v.lens = p->lens, v.refs = p->refs, v.used = p->used, v.state = p->state, v.work = p->work;
+    v.es = p->dtype == COLI_HIP_F32 ? 4 : 2;
+    v.n_layers = p->n_layers, v.KH = p->KH, v.hd = p->hd, v.page = p->page;
+    v.n_pages = p->n_pages, v.n_seqs = p->n_seqs, v.max_pages = p->max_pages;
+    v.row_bytes = (long)p->hd * v.es;
+    v.head_bytes = v.row_bytes * p->page;
+    v.kv_bytes = v.head_bytes * p->KH;
+    v.layer_bytes = 2 * v.kv_bytes;
+    v.page_bytes = v.layer_bytes * p->n_layers;
+    return true;
+}
+
+bool paged_stream(void *stream_, hipStream_t &st) {
+    if (!ok()) return false;
+    int dev = -1;
+    if (hipGetDevice(&dev) != hipSuccess || dev != 0) return paged_refuse("the library's device is not current");
+    st = stream_ ? (hipStream_t)stream_ : stream();
+    return true;
+}
+
+static bool launched(const char *what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess || fail(what, e);
+}
+
+// ---------------------------------------------------------------- block helpers
+// Exclusive prefix sum of v over the block's threads, the total in *total.
+__device__ __forceinline__ int block_scan(int v, int *s_wave, int *total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 63) s_wave[wave] = x;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < kPgThreads / 64; w++) {
+        const int t = s_wave[w];
+        before += w < wave ? t : 0;
+        all += t;
+    }
+    __syncthreads();
+    *total = all;
+    return before + x - v;
+}
+
+// The pages of word w that are in use; those past the pool's end count as used.
+__device__ __forceinline__ unsigned used_word(const PoolView &p, int w) {
+    unsigned u = p.used[w];
+    const int left = p.n_pages - w * 32;
+    if (left < 32) u |= ~0u << left;
+    return u;
+}
+
+__device__ __forceinline__ int pages_of(int len, int page) { return (int)(((long)len + page - 1) / page); }
+
+// ---------------------------------------------------------------- taking pages
+enum { kTakeAppend = 0, kTakeShare = 1, kTakeCopy = 2 };
+
+// One block.  Append: sequence b[i] grows by count[i] positions (NULL: 1).  Fork: b[i] becomes
+// as long as a[i]; its new pages are the last, partly filled one (share) or all of them (copy).
+// Nothing changes unless the whole call can be done.
+__global__ __launch_bounds__(kPgThreads) void pages_take(PoolView p, const int *__restrict__ a,
+                                                         const int *__restrict__ b, const int *__restrict__ count,
+                                                         int n, int mode) {
+    __shared__ int s_off[kPgMaxN + 1];
+    __shared__ int s_wave[kPgThreads / 64];
+    __shared__ int s_err;
+    const int tid = threadIdx.x;
+    if (tid == 0) s_err = 0;
+    __syncthreads();
+    // what each needs; a mark per sequence finds the ones named twice
+    int err = 0;
+    for (int i = tid; i < n; i += kPgThreads) {
+        const int s = b[i], f = mode == kTakeAppend ? s : a[i];
+        int need = 0;
+        if (s < -1 || s >= p.n_seqs || f < -1 || f >= p.n_seqs) {
+            err |= kPgIndex;
+        } else if (s >= 0 && f >= 0) {
+            p.work[s] = i;
+            const int len = p.lens[s];
+            const long most = (long)p.max_pages * p.page;
+            if (len < 0 || len > most) err |= kPgIndex;
+            if (mode == kTakeAppend) {
+                const int c = count ? count[i] : 1;
+                if (c < 0)
+                    err |= kPgIndex;
+                else if ((long)len + c > most)
+                    err |= kPgRow;
+                else
+                    need = pages_of(len + c, p.page) - pages_of(len, p.page);
+            } else {
+                const int from = p.lens[f];
+                if (len != 0 || s == f) err |= kPgTwice;
+                if (from < 0 || from > most) err |= kPgIndex;
+                need = mode == kTakeCopy ? pages_of(from, p.page) : from % p.page != 0;
+            }
+        }
+        s_off[i] = need;
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += kPgThreads) {
+        const int s = b[i], f = mode == kTakeAppend ? s : a[i];
+        if (s >= 0 && f >= 0 && s < p.n_seqs && f < p.n_seqs && p.work[s] != i) err |= kPgTwice;
+    }
+    // free pages, and the need: each thread sums four neighbours (both at most n_pages, or an error)
+    const int words = (p.n_pages + 31) / 32;
+    int nfree = 0, total_free, total = 0;
+    for (int w = tid; w < words; w += kPgThreads) nfree += 32 - __popc(used_word(p, w));
+    block_scan(nfree, s_wave, &total_free);
+    int v[kPgMaxN / kPgThreads], mine = 0, full = 0;
+#pragma unroll
+    for (int k = 0; k < kPgMaxN / kPgThreads; k++) {
+        const int i = tid * (kPgMaxN / kPgThreads) + k;
+        v[k] = i < n ? s_off[i] : 0;
+        if (v[k] > total_free) full = 1, v[k] = 0;
+        mine += v[k];
+        if (mine > total_free) full = 1, mine = 0;   // keeps the sums below 2^31
+    }
+    // 1024 partial sums of at most 2^30 each: summed in 64 bits for the check
+    __shared__ unsigned long long s_total;
+    if (tid == 0) s_total = 0;
+    __syncthreads();
+    if (mine || full) atomicAdd(&s_total, (unsigned long long)mine + (full ? 1ull << 40 : 0));
+    if (err) atomicOr(&s_err, err);
+    __syncthreads();
+    if (tid == 0 && !s_err && s_total > (unsigned long long)total_free) s_err = kPgFull;
+    __syncthreads();
+    if (s_err) {
+        if (tid == 0) {
+            atomicOr(&p.state[kStErr], s_err);
+            p.state[kStGo] = 0;
+        }
+        return;
+    }
+    int at = block_scan(mine, s_wave, &total);
+#pragma unroll
+    for (int k = 0; k < kPgMaxN / kPgThreads; k++) {
+        const int i = tid * (kPgMaxN / kPgThreads) + k;
+        if (i < n) s_off[i] = at;
+        at += v[k];
+    }
+    if (tid == 0) s_off[n] = total;
+    __syncthreads();
+    // the lowest `total` free pages, in order, into the list
+    int *list = p.work + p.n_seqs;
+    for (int w0 = 0, base = 0; base < total && w0 < words; w0 += kPgThreads) {
+        const int w = w0 + tid;
+        unsigned fr = w < words ? ~used_word(p, w) : 0u;
+        int found;
+        int r = base + block_scan(__popc(fr), s_wave, &found);
+        unsigned taken = 0;
+        while (fr && r < total) {
+            const int bit = __ffs(fr) - 1;
+            list[r++] = w * 32 + bit;
+            taken |= 1u << bit;
+            fr &= fr - 1;
+        }
+        if (taken) p.used[w] |= taken;
+        base += found;
+    }
+    __syncthreads();
+    // each page to its table entry
+    for (int r = tid; r < total; r += kPgThreads) {
+        int lo = 0, hi = n;   // the last i with s_off[i] <= r
+        while (hi - lo > 1) {
+            const int m = (lo + hi) / 2;
+            if (s_off[m] <= r)
+                lo = m;
+            else
+                hi = m;
+        }
+        const int s = b[lo], k = r - s_off[lo], pg = list[r];
+        const int first = mode == kTakeAppend ? pages_of(p.lens[s], p.page)
+                        : mode == kTakeShare  ? p.lens[a[lo]] / p.page
+                                              : 0;
+        p.table[(size_t)s * p.max_pages + first + k] = pg;
+        p.refs[pg] = 1;
+    }
+    // the lengths, all read before the first is written: a fork's source may be another's target
+    int len[kPgMaxN / kPgThreads];
+#pragma unroll
+    for (int k = 0; k < kPgMaxN / kPgThreads; k++) {
+        const int i = tid + k * kPgThreads;
+        len[k] = -1;
+        if (i >= n) continue;
+        const int s = b[i], f = mode == kTakeAppend ? s : a[i];
+        if (s < 0 || f < 0) continue;
+        len[k] = mode == kTakeAppend ? p.lens[s] + (count ? count[i] : 1) : p.lens[f];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kPgMaxN / kPgThreads; k++)
+        if (len[k] >= 0) p.lens[b[tid + k * kPgThreads]] = len[k];
+    if (tid == 0) p.state[kStGo] = 1;
+}
+
+// ---------------------------------------------------------------- copying
+// The first `held` rows of every head plane of page `from` to page `to`, piece of pieces.
+__device__ __forceinline__ void copy_page(const PoolView &p, int from, int to, int held, int piece, int pieces) {
+    const uint4 *src = (const uint4 *)(p.data + (size_t)from * p.page_bytes);
+    uint4 *dst = (uint4 *)(p.data + (size_t)to * p.page_bytes);
+    const long row16 = p.row_bytes / 16;
+    if (held == p.page) {
+        const long n = p.page_bytes / 16, per = (n + pieces - 1) / pieces;
+        const long end = min(n, (piece + 1) * per);
+        for (long u = piece * per + threadIdx.x; u < end; u += blockDim.x) dst[u] = src[u];
+        return;
+    }
+    const long plane = held * row16, n = plane * p.n_layers * 2 * p.KH, stride = p.head_bytes / 16;
+    const long per = (n + pieces - 1) / pieces, end = min(n, (piece + 1) * per);
+    for (long u = piece * per + threadIdx.x; u < end; u += blockDim.x) {
+        const long at = u / plane * stride + u % plane;
+        dst[at] = src[at];
+    }
+}
+
+static int pieces_of(const PoolView &p) {
+    const long n = (p.page_bytes + kCopyPiece - 1) / kCopyPiece;
+    return (int)(n < 1 ? 1 : n > 4096 ? 4096 : n);
+}
+
+// Behind pages_take: the shared entries of the table with their counts, and the rows of the
+// new pages.  Block (i, y) takes every gridDim.y-th piece of pair i.
+__global__ __launch_bounds__(kCopyThreads) void pages_fork_copy(PoolView p, const int *__restrict__ a,
+                                                                const int *__restrict__ b, int share, int pieces) {
+    const int s = b[blockIdx.x], f = a[blockIdx.x];
+    if (!p.state[kStGo] || s < 0 || f < 0) return;
+    const int len = p.lens[s], full = len / p.page, np = pages_of(len, p.page);
+    const int *from = p.table + (size_t)f * p.max_pages;
+    int *to = p.table + (size_t)s * p.max_pages;
+    if (share)
+        for (int j = blockIdx.y * kCopyThreads + threadIdx.x; j < full; j += gridDim.y * kCopyThreads) {
+            const int pg = from[j];
+            to[j] = pg;
+            if (pg >= 0 && pg < p.n_pages)
+                atomicAdd(&p.refs[pg], 1);
+            else
+                atomicOr(&p.state[kStErr], kPgPage);
+        }
+    const int j0 = share ? full : 0;
+    const long tasks = (long)(np - j0) * pieces;
+    for (long t = blockIdx.y; t < tasks; t += gridDim.y) {
+        const int j = j0 + (int)(t / pieces), src = from[j], dst = to[j];
+        if (src < 0 || src >= p.n_pages || dst < 0 || dst >= p.n_pages) {
+            atomicOr(&p.state[kStErr], kPgPage);
+            continue;
+        }
+        copy_page(p, src, dst, min(p.page, len - j * p.page), (int)(t % pieces), pieces);
+    }
+}
+
+// ---------------------------------------------------------------- freeing
+// Block i ends sequence seq[i]: the length is taken atomically, so a sequence named twice (or
+// an empty one) is freed once.
+__global__ __launch_bounds__(kCopyThreads) void pages_drop(PoolView p, const int *__restrict__ seq) {
+    __shared__ int s_len;
+    const int s = seq[blockIdx.x];
+    if (s < 0 || s >= p.n_seqs) {
+        if (s != -1 && threadIdx.x == 0) atomicOr(&p.state[kStErr], kPgIndex);
+        return;
+    }
+    if (threadIdx.x == 0) s_len = atomicExch(&p.lens[s], 0);
+    __syncthreads();
+    const int np = min(pages_of(s_len, p.page), p.max_pages);
+    int *row = p.table + (size_t)s * p.max_pages;
+    for (int j = threadIdx.x; j < np; j += kCopyThreads) {
+        const int pg = row[j];
+        row[j] = -1;
+        if (pg < 0 || pg >= p.n_pages) {
+            atomicOr(&p.state[kStErr], kPgPage);
+            continue;
+        }
+        if (atomicSub(&p.refs[pg], 1) == 1) atomicAnd(&p.used[pg >> 5], ~(1u << (pg & 31)));
+    }
+}
+
+// ---------------------------------------------------------------- closing up
+// One block: with L pages in use, the k-th used page at or past L (a mover) goes into the k-th
+// free page below L (a hole).  work holds the holes, the movers, and for each page past L its
+// new place.
+__global__ __launch_bounds__(kPgThreads) void pages_plan(PoolView p) {
+    __shared__ int s_wave[kPgThreads / 64];
+    const int tid = threadIdx.x, words = (p.n_pages + 31) / 32;
+    int n = 0, live;
+    for (int w = tid; w < words; w += kPgThreads) n += 32 - __popc(used_word(p, w));
+    block_scan(n, s_wave, &live);
+    live = p.n_pages - live;
+    int *hole = p.work + p.n_seqs, *mover = hole + (p.n_pages + 1) / 2 + 1, *to = hole + p.n_pages + 4;
+    int nh = 0, nm = 0;
+    for (int w0 = 0; w0 < words; w0 += kPgThreads) {
+        const int w = w0 + tid;
+        const unsigned u = w < words ? used_word(p, w) : 0u;
+        const int below = live - w * 32;   // this word's pages below L
+        const unsigned low = below >= 32 ? ~0u : below <= 0 ? 0u : (1u << below) - 1u;
+        unsigned h = w < words ? ~u & low : 0u, m = u & ~low;
+        const int left = p.n_pages - w * 32;   // the last word's bits past the end are no pages
+        if (left < 32) m &= left <= 0 ? 0u : (1u << left) - 1u;
+        int got;
+        int r = nh + block_scan(__popc(h), s_wave, &got);
+        nh += got;
+        while (h) {
+            hole[r++] = w * 32 + __ffs(h) - 1;
+            h &= h - 1;
+        }
+        r = nm + block_scan(__popc(m), s_wave, &got);
+        nm += got;
+        while (m) {
+            mover[r++] = w * 32 + __ffs(m) - 1;
+            m &= m - 1;
+        }
+        if (w < words) p.used[w] = low;
+    }
+    __syncthreads();
+    for (int k = tid; k < nm; k += kPgThreads) {
+        const int h = hole[k], m = mover[k];
+        to[m - live] = h;
+        p.refs[h] = p.refs[m];
+        p.refs[m] = 0;
+    }
+    if (tid == 0) {
+        p.state[kStMove] = nm;
+        p.state[kStLive] = live;
+    }
+}
+
+__global__ __launch_bounds__(kCopyThreads) void pages_move(PoolView p, int pieces) {
+    const int moved = p.state[kStMove], live = p.state[kStLive];
+    if (!moved) return;
+    const int *hole = p.work + p.n_seqs, *mover = hole + (p.n_pages + 1) / 2 + 1, *to = hole + p.n_pages + 4;
+    const long tasks = (long)moved * pieces;
+    for (long t = blockIdx.x; t < tasks; t += gridDim.x) {
+        const int k = (int)(t / pieces);
+        copy_page(p, mover[k], hole[k], p.page, (int)(t % pieces), pieces);
+    }
+    for (int s = blockIdx.x; s < p.n_seqs; s += gridDim.x) {
+        const int np = min(pages_of(p.lens[s], p.page), p.max_pages);
+        int *row = p.table + (size_t)s * p.max_pages;
+        for (int j = threadIdx.x; j < np; j += kCopyThreads) {
+            const int pg = row[j];
+            if (pg >= p.n_pages || pg < 0)
+                atomicOr(&p.state[kStErr], kPgPage);
+            else if (pg >= live)
+                row[j] = to[pg - live];
+        }
+    }
+}
+
+// ---------------------------------------------------------------- a new pool
+__global__ __launch_bounds__(256) void pages_clear(PoolView p) {
+    const size_t i0 = blockIdx.x * 256 + threadIdx.x, step = (size_t)gridDim.x * 256;
+    for (size_t i = i0; i < (size_t)p.n_seqs * p.max_pages; i += step) p.table[i] = -1;
+    for (size_t i = i0; i < (size_t)p.n_seqs; i += step) p.lens[i] = 0;
+    for (size_t i = i0; i < (size_t)p.n_pages; i += step) p.refs[i] = 0;
+    for (size_t i = i0; i < (size_t)(p.n_pages + 31) / 32; i += step) p.used[i] = 0;
+    for (size_t i = i0; i < COLI_HIP_PAGES_STATE; i += step) p.state[i] = 0;
+}
+
+}  // namespace coli
+
+using namespace coli;
+
+COLI_API int coli_hip_pages_check(const ColiHipPages *p) {
+    PoolView v;
+    return pool_view(p, v) ? 1 : 0;
+}
+
+COLI_API size_t coli_hip_pages_work(const ColiHipPages *p) {
+    return p && p->n_seqs > 0 && p->n_pages > 0 ? (size_t)p->n_seqs + 2 * (size_t)p->n_pages + 64 : 0;
+}
+
+COLI_API int coli_hip_pages_init(const ColiHipPages *p, void *stream_) {
+    PoolView v;
+    hipStream_t st;
+    if (!pool_view(p, v) || !paged_stream(stream_, st)) return 0;
+    const size_t most = (size_t)v.n_seqs * v.max_pages, all = most > (size_t)v.n_pages ? most : v.n_pages;
+    const unsigned grid = (unsigned)(all / 256 + 1 < 2048 ? all / 256 + 1 : 2048);
+    hipLaunchKernelGGL(pages_clear, dim3(grid), dim3(256), 0, st, v);
+    return launched("pages init") ? 1 : 0;
+}
+
+static bool take_args(const ColiHipPages *p, PoolView &v, const void *seq, int n) {
+    if (!pool_view(p, v)) return false;
+    if (n < 0 || n > kPgMaxN) return paged_refuse("more than 4096 sequences in a call");
+    return !n || seq || paged_refuse("NULL sequence list");
+}
+
+COLI_API int coli_hip_pages_append(const ColiHipPages *p, const int *d_seq, const int *d_count, int n, void *stream_) {
+    PoolView v;
+    hipStream_t st;
+    if (!take_args(p, v, d_seq, n) || !paged_stream(stream_, st)) return 0;
+    if (!n) return 1;
+    hipLaunchKernelGGL(pages_take, dim3(1), dim3(kPgThreads), 0, st, v, d_seq, d_seq, d_count, n, (int)kTakeAppend);
+    return launched("pages append") ? 1 : 0;
+}
+
+COLI_API int coli_hip_pages_fork(const ColiHipPages *p, const int *d_src, const int *d_dst, int n, int share,
+                                 void *stream_) {
+    PoolView v;
+    hipStream_t st;
+    if (!take_args(p, v, d_src && d_dst ? d_src : nullptr, n) || !paged_stream(stream_, st)) return 0;
+    if (!n) return 1;
+    hipLaunchKernelGGL(pages_take, dim3(1), dim3(kPgThreads), 0, st, v, d_src, d_dst, (const int *)nullptr, n,
+                       share ? (int)kTakeShare : (int)kTakeCopy);
+    const int pieces = pieces_of(v);
+    // share: a page's pieces; copy: enough blocks for the whole card
+    long y = share ? pieces : (8L * n_cu() + n - 1) / n;
+    y = y < 1 ? 1 : y > 2048 ? 2048 : y;
+    hipLaunchKernelGGL(pages_fork_copy, dim3(n, (unsigned)y), dim3(kCopyThreads), 0, st, v, d_src, d_dst, share ? 1 : 0,
+                       pieces);
+    return launched("pages fork") ? 1 : 0;
+}
+
+COLI_API int coli_hip_pages_free(const ColiHipPages *p, const int *d_seq, int n, void *stream_) {
+    PoolView v;
+    hipStream_t st;
+    if (!take_args(p, v, d_seq, n) || !paged_stream(stream_, st)) return 0;
+    if (!n) return 1;
+    hipLaunchKernelGGL(pages_drop, dim3(n), dim3(kCopyThreads), 0, st, v, d_seq);
+    return launched("pages free") ? 1 : 0;
+}
+
+COLI_API int coli_hip_pages_compact(const ColiHipPages *p, void *stream_) {
+    PoolView v;
+    hipStream_t st;
+    if (!pool_view(p, v) || !paged_stream(stream_, st)) return 0;
+    hipLaunchKernelGGL(pages_plan, dim3(1), dim3(kPgThreads), 0, st, v);
+    hipLaunchKernelGGL(pages_move, dim3(8 * n_cu()), dim3(kCopyThreads), 0, st, v, pieces_of(v));
+    return launched("pages compact") ? 1 : 0;
+}
+
+COLI_API int coli_hip_pages_status(const ColiHipPages *p, int *n_free, int *errors, void *stream_) {
+    PoolView v;
+    hipStream_t st;
+    if (!pool_view(p, v) || !paged_stream(stream_, st)) return 0;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(st, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone)
+        return paged_refuse("a status read in a captured stream") ? 1 : 0;
+    const int words = (v.n_pages + 31) / 32;
+    unsigned *h = (unsigned *)malloc((size_t)words * 4);
+    if (!h) return 0;
+    int err = 0;
+    const int zero = 0;
+    hipError_t e = hipMemcpyAsync(h, v.used, (size_t)words * 4, hipMemcpyDeviceToHost, st);
+    if (e == hipSuccess) e = hipMemcpyAsync(&err, v.state + kStErr, 4, hipMemcpyDeviceToHost, st);
+    if (e == hipSuccess) e = hipStreamSynchronize(st);
+    if (e == hipSuccess && err) e = hipMemcpyAsync(v.state + kStErr, &zero, 4, hipMemcpyHostToDevice, st);
+    if (e == hipSuccess && err) e = hipStreamSynchronize(st);
+    int fr = 0;
+    for (int w = 0; e == hipSuccess && w < words; w++) {
+        const int left = v.n_pages - w * 32;
+        fr += __builtin_popcount(~h[w] & (left < 32 ? (1u << left) - 1u : ~0u));
+    }
+    free(h);
+    if (e != hipSuccess) return fail("pages status", e) ? 1 : 0;
+    if (n_free) *n_free = fr;
+    if (errors) *errors = err;
+    return 1;
+}

@@ -594,6 +594,7 @@ COLI_API void coli_vk_shutdown(void) {
     prefill_shutdown();
     layer_shutdown();
     container_shutdown();
+    paged_shutdown();
     read_back_shutdown();
     scratch_free(&g_stage, &g_stage_cap);
     for (int i = 0; i < G.nblocks; i++) (void)hipFree(G.blocks[i].base);
