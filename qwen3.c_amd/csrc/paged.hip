@@ -142,62 +142,385 @@ __global__ __launch_bounds__(64) void qk_rope_rows(PoolView p, HeadsView h, int 
 }
 
 // ---------------------------------------------------------------- attention over pages
-// o = sum_t softmax_t(scale q . k_t) v_t over t <= pos, one pass with the running maximum m and
-// sum l; a block per (row, query head), its waves take the keys in turn, a wave holds four
-// columns per lane.
-constexpr int kRowWaves = 16;
+// o = sum_t softmax_t(scale q . k_t) v_t over t <= pos, one pass with a running maximum m and
+// sum l per head (scores in units of log 2, the scale and log2 e folded into q).
+//
+// The products run on v_mfma_f32_16x16x4_f32 with the pages' values widened to 32 bits (exact), a
+// wave on 16 keys of one kv head and up to 16 of its query heads at a time:
+//   scores [key][head] = K q^T: A[key l % 16][k = l / 16], one 16-byte load of the lane's key row
+//     is the operand of 4 (f32) or 8 products; lane l ends up with keys 4 (l / 16) + i of head
+//     l % 16.
+//   out [head][column] += P V: the lane's own weight i is A[head l % 16][k = l / 16] for key
+//     4 k + i; B[k][column] is the lane's 16-byte piece of that key's row, so product n of a
+//     piece covers columns n, n + 8, ..: no transpose, no LDS but for q.
+//
+// Work: row r's unit is kKeys keys of a kv head, kWaves tiles side by side; the units of all rows
+// in one line are cut into equal shares, one per block, whatever the lengths are.  A block's part
+// of a (row, kv head) that it does not hold whole goes to the workspace, and attn_join puts the
+// parts together.
+constexpr int kTile = 16, kWaves = 4, kKeys = kTile * kWaves, kGroup = 16;   // kGroup: heads a wave takes
+constexpr int kAttnBlocks = 512;   // two blocks per CU
+constexpr int kAttnThreads = 64 * kWaves;
+constexpr float kLazy = 8.f;   // the maximum is moved when a score passes it by 2^8: weights stay below
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+struct PagedArgs {
+    const float *q, *gate;
+    const int *seq, *pos;
+    float *out, *part;
+    float2 *ml;
+    int n, layer, groups, khv;   // head groups of kGroup per kv head, khv = KH * groups
+    unsigned magic, shift;       // t / page = (umulhi(t, magic) + t) >> shift, t < 2^31
+};
+
+// The positions that row r sees (a row of no sequence: -1).
+__device__ __forceinline__ int row_count(const PoolView &p, const PagedArgs &a, int r, int &s) {
+    const int at = row_pos(p, a.seq, a.pos, r, s);
+    return s < 0 ? -1 : at < -2 ? -3 - at : at < 0 ? 0 : at + 1;   // past the end: what is held
+}
+__device__ __forceinline__ int chunks_of(int cnt) { return cnt < 1 ? cnt + 1 : (int)(((unsigned)cnt + kKeys - 1) / kKeys); }
+
+// The units of all rows in one line.  s_base[t]: the units before the rows of thread t.
+struct Line {
+    long total, share;
+    int per;
+};
+__device__ __forceinline__ Line line_up(const PoolView &p, const PagedArgs &a, int nblocks, long *s_base, long *s_wave) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    Line l;
+    l.per = (a.n + kAttnThreads - 1) / kAttnThreads;
+    long mine = 0;
+    for (int i = 0; i < l.per; i++) {
+        const int r = tid * l.per + i;
+        int s;
+        if (r < a.n) mine += (long)chunks_of(row_count(p, a, r, s)) * a.khv;
+    }
+    long x = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 63) s_wave[wave] = x;
+    __syncthreads();
+    long before = 0;
+    l.total = 0;
+    for (int w = 0; w < kWaves; w++) {
+        before += w < wave ? s_wave[w] : 0;
+        l.total += s_wave[w];
+    }
+    s_base[tid] = before + x - mine;
+    l.share = (l.total + nblocks - 1) / nblocks;
+    if (l.share < 1) l.share = 1;
+    __syncthreads();
+    return l;
+}
+// The row of unit u < total: r, its first unit.
+__device__ __forceinline__ int row_of(const PoolView &p, const PagedArgs &a, const Line &l, const long *s_base, long u,
+                                      long &first) {
+    int lo = 0, hi = kAttnThreads;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) / 2;
+        if (s_base[m] <= u)
+            lo = m;
+        else
+            hi = m;
+    }
+    int r = lo * l.per;
+    first = s_base[lo];
+    for (; r < a.n; r++) {
+        int s;
+        const long k = (long)chunks_of(row_count(p, a, r, s)) * a.khv;
+        if (first + k > u) break;
+        first += k;
+    }
+    return r;   // n only if the lengths change under the kernel
+}
+
 template <int T>
-__global__ __launch_bounds__(64 * kRowWaves) void attn_rows(PoolView p, HeadsView h, int layer, const float *__restrict__ q,
-                                                 const float *__restrict__ gate, const int *__restrict__ seq,
-                                                 const int *__restrict__ pos, float *__restrict__ out) {
-    using D = typename Val<T>::type;
-    __shared__ float s_m[kRowWaves], s_l[kRowWaves], s_o[kRowWaves][256];
-    const int n = blockIdx.x, hq = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int s;
-    int at = row_pos(p, seq, pos, n, s);
-    if (s < 0) return;
-    if (at < -2) at = -4 - at;   // past the end: what the sequence holds
-    const int cnt = at < 0 ? 0 : at + 1, kh = hq / (h.H / p.KH), d0 = lane * 4;
-    const bool in = d0 < p.hd;
-    float x[4] = {}, acc[4] = {}, m = -INFINITY, l = 0.f;
-    for (int i = 0; i < 4 && in; i++) x[i] = q[((size_t)n * h.H + hq) * p.hd + d0 + i];
-    const int *row = p.table + (size_t)s * p.max_pages;
-    for (int t = wave; t < cnt; t += kRowWaves) {
-        const int pg = row[t / p.page];
-        if (pg < 0 || pg >= p.n_pages) {
-            if (lane == 0) atomicOr(&p.state[kStErr], kPgPage);
+__device__ __forceinline__ void widen(const uint4 &x, float *f) {
+    const unsigned w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (T == COLI_HIP_F32) {
+            f[i] = __uint_as_float(w[i]);
+        } else if (T == COLI_HIP_BF16) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+            f[2 * i] = (float)__builtin_bit_cast(_Float16, (unsigned short)w[i]);
+            f[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(w[i] >> 16));
+        }
+    }
+}
+
+// max / sum over the four lanes that hold a head's keys (l, l ^ 16, l ^ 32, l ^ 48)
+__device__ __forceinline__ float max4(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float sum4(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+template <int T, int HD, bool kExact>
+__global__ __launch_bounds__(kAttnThreads, 2) void attn_part(PoolView p, HeadsView h, PagedArgs a) {
+    constexpr int kE = T == COLI_HIP_F32 ? 4 : 8;          // values of a 16-byte piece
+    constexpr int kKC = HD / (4 * kE), kVS = HD / (16 * kE) < 1 ? 1 : HD / (16 * kE);
+    constexpr int kQ = HD + 4;                             // row of q in LDS
+    __shared__ long s_base[kAttnThreads], s_wave[kWaves];
+    __shared__ float s_q[kGroup * kQ];
+    __shared__ float s_m[kWaves][kGroup], s_l[kWaves][kGroup];
+    __shared__ float s_o[2][kVS * kE * 256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int G = h.H / p.KH, pieces = (int)(p.row_bytes / 16);
+    const Line ln = line_up(p, a, gridDim.x, s_base, s_wave);
+    const long u0 = blockIdx.x * ln.share, end = min(ln.total, u0 + ln.share);
+    if (u0 >= end) return;
+    long first;
+    int r = row_of(p, a, ln, s_base, u0, first);
+    for (long u = u0; u < end && r < a.n;) {
+        int s;
+        const int cnt = row_count(p, a, r, s), nc = chunks_of(cnt);
+        const long x = u - first;
+        if (x >= (long)nc * a.khv) {   // this row is done (or has none)
+            first += (long)nc * a.khv;
+            r++;
             continue;
         }
-        const D *K = (const D *)(p.data + (size_t)pg * p.page_bytes + layer * p.layer_bytes + kh * p.head_bytes +
-                                 (t % p.page) * p.row_bytes);
-        const D *V = (const D *)((const char *)K + p.kv_bytes);
-        float dot = 0.f;
-        for (int i = 0; i < 4 && in; i++) dot = fmaf(x[i], Val<T>::up(K[d0 + i]), dot);
-        for (int o = 32; o; o >>= 1) dot += __shfl_xor(dot, o);
-        dot *= h.scale;
-        const float nm = fmaxf(m, dot);
-        const float f = m == nm ? 1.f : expf(m - nm), w = dot == -INFINITY ? 0.f : expf(dot - nm);
-        for (int i = 0; i < 4 && in; i++) acc[i] = fmaf(acc[i], f, w * Val<T>::up(V[d0 + i]));
-        l = fmaf(l, f, w);
-        m = nm;
+        const int hv = (int)(x / nc), c0 = (int)(x % nc), c1 = (int)min((long)nc, c0 + (end - u));
+        const int kh = hv / a.groups, h0 = (hv % a.groups) * kGroup, hn = min(kGroup, G - h0);
+        const long head = (long)kh * G + h0;   // first query head
+        // q, scaled, zero past the last head and column
+        const float *q = a.q + ((long)r * h.H + head) * p.hd;
+        const float qs = h.scale * 1.4426950408889634f;
+        for (int i = tid; i < kGroup * HD; i += kAttnThreads) {
+            const int hh = i / HD, d = i % HD;
+            s_q[hh * kQ + d] = hh < hn && (kExact || d < p.hd) ? q[hh * p.hd + d] * qs : 0.f;
+        }
+        __syncthreads();
+        v4f acc[kVS * kE];
+#pragma unroll
+        for (int i = 0; i < kVS * kE; i++) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+        const int *row = p.table + (size_t)s * p.max_pages;
+        const char *base = p.data + (size_t)a.layer * p.layer_bytes + (size_t)kh * p.head_bytes;
+        const int last = min(cnt, c1 * kKeys);
+        // the lane's key of a tile: its page, then where its row lies
+        auto page_id = [&](int key0) {
+            const unsigned t = (unsigned)min(key0 + c, cnt - 1);
+            return row[(__umulhi(t, a.magic) + t) >> a.shift];
+        };
+        auto locate = [&](int key0, int pg, long &off) {
+            const unsigned t = (unsigned)min(key0 + c, cnt - 1), j = (__umulhi(t, a.magic) + t) >> a.shift;
+            const bool is = pg >= 0 && pg < p.n_pages;
+            if (!is && key0 + c < cnt) atomicOr(&p.state[kStErr], kPgPage);
+            off = (is ? (long)pg * p.page_bytes : 0) + (long)(t - j * p.page) * p.row_bytes;
+            return is && key0 + c < cnt;
+        };
+        uint4 kb[kKC], vb[4][kVS];
+        auto load_k = [&](long off) {
+            const uint4 *k = (const uint4 *)(base + off) + g;
+#pragma unroll
+            for (int i = 0; i < kKC; i++) {
+                kb[i] = uint4{0, 0, 0, 0};
+                if (kExact || 4 * i + g < pieces) kb[i] = k[4 * i];
+            }
+        };
+        auto load_v = [&](long off) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const long o = __shfl(off, 4 * g + j);
+                const uint4 *v = (const uint4 *)(base + p.kv_bytes + o) + c;
+#pragma unroll
+                for (int i = 0; i < kVS; i++) {
+                    vb[j][i] = uint4{0, 0, 0, 0};
+                    if ((kExact && HD >= 16 * kE) || 16 * i + c < pieces) vb[j][i] = v[16 * i];
+                }
+            }
+        };
+        int key0 = c0 * kKeys + wave * kTile;
+        long off = 0, off_next = 0;
+        bool valid = false, valid_next = false;
+        int pg_next = 0;
+        if (key0 < last) {
+            valid = locate(key0, page_id(key0), off);
+            load_k(off);
+            load_v(off);
+            if (key0 + kKeys < last) pg_next = page_id(key0 + kKeys);
+        }
+        for (; key0 < last; key0 += kKeys) {
+            const bool more = key0 + kKeys < last;
+            const unsigned vm = (unsigned)(__ballot(valid) & 0xffff);
+            v4f sc = {0.f, 0.f, 0.f, 0.f}, sd = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < kKC; i++) {
+                float kf[8];
+                widen<T>(kb[i], kf);
+                const float *qp = s_q + c * kQ + (4 * i + g) * kE;
+                float qf[kE];
+#pragma unroll
+                for (int j = 0; j < kE; j += 4) *(float4 *)(qf + j) = *(const float4 *)(qp + j);
+#pragma unroll
+                for (int j = 0; j < kE; j += 2) {
+                    sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[j], sc, 0, 0, 0);
+                    sd = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j + 1], qf[j + 1], sd, 0, 0, 0);
+                }
+            }
+            if (more) {
+                valid_next = locate(key0 + kKeys, pg_next, off_next);
+                load_k(off_next);
+                if (key0 + 2 * kKeys < last) pg_next = page_id(key0 + 2 * kKeys);
+            }
+            sc += sd;
+            if (vm != 0xffff) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (vm >> (4 * g + i) & 1) continue;
+                    sc[i] = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < kVS; j++) vb[i][j] = uint4{0, 0, 0, 0};
+                }
+            }
+            const float mt = max4(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
+            if (__any(mt > m + kLazy || (m == -INFINITY && mt > m))) {
+                const float nm = fmaxf(m, mt), f = m == nm ? 1.f : __builtin_amdgcn_exp2f(m - nm);
+                l *= f;
+                m = nm;
+                float fr[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) fr[i] = __shfl(f, 4 * g + i);
+#pragma unroll
+                for (int t = 0; t < kVS * kE; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[t][i] *= fr[i];
+            }
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = sc[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sc[i] - m);
+            l += (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+#pragma unroll
+                for (int i = 0; i < kVS; i++) {
+                    float vf[8];
+                    widen<T>(vb[j][i], vf);
+#pragma unroll
+                    for (int e = 0; e < kE; e++)
+                        acc[i * kE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], vf[e], acc[i * kE + e], 0, 0, 0);
+                }
+            }
+            if (more) {
+                load_v(off_next);
+                off = off_next;
+                valid = valid_next;
+            }
+        }
+        // the four waves' parts: one maximum, then the sums pairwise through LDS
+        l = sum4(l);
+        if (g == 0) {
+            s_m[wave][c] = m;
+            s_l[wave][c] = l;
+        }
+        __syncthreads();
+        float M[4], f[4], L[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int hh = 4 * g + i;
+            M[i] = fmaxf(fmaxf(s_m[0][hh], s_m[1][hh]), fmaxf(s_m[2][hh], s_m[3][hh]));
+            L[i] = 0.f;
+            for (int w = 0; w < kWaves; w++) {
+                const float mw = s_m[w][hh], fw = mw == M[i] ? 1.f : __builtin_amdgcn_exp2f(mw - M[i]);
+                L[i] += s_l[w][hh] * fw;
+                if (w == wave) f[i] = fw;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kVS * kE; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[t][i] *= f[i];
+#pragma unroll
+        for (int step = 2; step; step >>= 1) {
+            if (wave >= step && wave < 2 * step) {
+#pragma unroll
+                for (int t = 0; t < kVS * kE; t++) *(v4f *)&s_o[wave - step][(t * 64 + lane) * 4] = acc[t];
+            }
+            __syncthreads();
+            if (wave < step) {
+#pragma unroll
+                for (int t = 0; t < kVS * kE; t++) acc[t] += *(const v4f *)&s_o[wave][(t * 64 + lane) * 4];
+            }
+            __syncthreads();
+        }
+        if (wave == 0) {
+            const bool whole = c0 == 0 && c1 == nc;
+            const long slot = 2L * blockIdx.x + (u == u0 ? 0 : 1);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int hh = 4 * g + i;
+                if (hh >= hn) continue;
+                float *dst = whole ? a.out + ((long)r * h.H + head + hh) * p.hd : a.part + (slot * kGroup + hh) * p.hd;
+                const float *gt = a.gate ? a.gate + r * h.q_row + (head + hh) * h.q_head : nullptr;
+                const float inv = cnt ? 1.f / L[i] : 0.f;
+                if (!whole && c == 0) a.ml[slot * kGroup + hh] = make_float2(M[i], L[i]);
+#pragma unroll
+                for (int j = 0; j < kVS; j++) {
+                    if (!(kExact && HD >= 16 * kE) && 16 * j + c >= pieces) continue;
+                    float o[kE];
+                    const int d0 = (16 * j + c) * kE;
+#pragma unroll
+                    for (int e = 0; e < kE; e++) {
+                        o[e] = acc[j * kE + e][i];
+                        if (whole) {
+                            o[e] = cnt ? o[e] * inv : 0.f;
+                            if (gt) o[e] /= 1.f + expf(-gt[d0 + e]);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < kE; e += 4) *(float4 *)(dst + d0 + e) = *(const float4 *)(o + e);
+                }
+            }
+        }
+        u += c1 - c0;
     }
-    if (in)
-        for (int i = 0; i < 4; i++) s_o[wave][d0 + i] = acc[i];
-    if (lane == 0) s_m[wave] = m, s_l[wave] = l;
-    __syncthreads();
-    float M = -INFINITY, L = 0.f, f[kRowWaves];
-    for (int w = 0; w < kRowWaves; w++) M = fmaxf(M, s_m[w]);
-    for (int w = 0; w < kRowWaves; w++) {
-        f[w] = s_m[w] == M ? 1.f : expf(s_m[w] - M);
-        L += f[w] * s_l[w];
+}
+
+// Block (j, hh): the (row, kv head) that the border between blocks j and j + 1 of attn_part
+// cuts, when it is the first border inside it: head hh of its parts joined.
+__global__ __launch_bounds__(kAttnThreads) void attn_join(PoolView p, HeadsView h, PagedArgs a, int nblocks) {
+    __shared__ long s_base[kAttnThreads], s_wave[kWaves];
+    const Line ln = line_up(p, a, nblocks, s_base, s_wave);
+    const long u = (blockIdx.x + 1L) * ln.share;
+    if (u >= ln.total) return;
+    long first;
+    const int r = row_of(p, a, ln, s_base, u, first);
+    if (r >= a.n) return;
+    int s;
+    const int nc = chunks_of(row_count(p, a, r, s)), G = h.H / p.KH;
+    const int hv = (int)((u - first) / nc), hh = blockIdx.y;
+    const long from = first + (long)hv * nc, to = from + nc;   // its units
+    if (from == u || from < u - ln.share) return;              // not cut here, or cut before
+    const int h0 = (hv % a.groups) * kGroup;
+    if (hh >= min(kGroup, G - h0)) return;
+    const long head = (long)(hv / a.groups) * G + h0 + hh;
+    const long b0 = from / ln.share, b1 = (to - 1) / ln.share;
+    auto slot_of = [&](long b) { return (2 * b + (from <= b * ln.share ? 0 : 1)) * kGroup + hh; };
+    float M = -INFINITY, L = 0.f;
+    for (long b = b0; b <= b1; b++) M = fmaxf(M, a.ml[slot_of(b)].x);
+    const int d = threadIdx.x;
+    float o = 0.f;
+    for (long b = b0; b <= b1; b++) {
+        const float2 ml = a.ml[slot_of(b)];
+        const float f = ml.x == M ? 1.f : __builtin_amdgcn_exp2f(ml.x - M);
+        L += f * ml.y;
+        if (d < p.hd) o += f * a.part[slot_of(b) * p.hd + d];
     }
-    for (int d = threadIdx.x; d < p.hd; d += 64 * kRowWaves) {
-        float o = 0.f;
-        for (int w = 0; w < kRowWaves; w++) o += f[w] * s_o[w][d];
-        o = cnt ? o / L : 0.f;
-        if (gate) o /= 1.f + expf(-gate[n * h.q_row + hq * h.q_head + d]);
-        out[((size_t)n * h.H + hq) * p.hd + d] = o;
-    }
+    if (d >= p.hd) return;
+    o /= L;
+    if (a.gate) o /= 1.f + expf(-a.gate[r * h.q_row + head * h.q_head + d]);
+    a.out[((long)r * h.H + head) * p.hd + d] = o;
 }
 
 static bool rows_args(const ColiHipPages *p, int layer, int n) {
@@ -222,20 +545,49 @@ static bool rope_launch(const PoolView &pv, const HeadsView &hv, int dtype, int 
     return launched("qk rope launch");
 }
 
+static size_t attn_work(const PoolView &pv) {
+    return 2 * (size_t)kAttnBlocks * kGroup * (pv.hd * sizeof(float) + sizeof(float2));
+}
+
+template <int T>
+static void attn_launch_t(const PoolView &pv, const HeadsView &hv, const PagedArgs &a, int blocks, hipStream_t st) {
+    const dim3 g(blocks), t(kAttnThreads);
+    switch (pv.hd) {
+    case 64: hipLaunchKernelGGL((attn_part<T, 64, true>), g, t, 0, st, pv, hv, a); return;
+    case 128: hipLaunchKernelGGL((attn_part<T, 128, true>), g, t, 0, st, pv, hv, a); return;
+    case 256: hipLaunchKernelGGL((attn_part<T, 256, true>), g, t, 0, st, pv, hv, a); return;
+    }
+    if (pv.hd < 64)
+        hipLaunchKernelGGL((attn_part<T, 64, false>), g, t, 0, st, pv, hv, a);
+    else if (pv.hd < 128)
+        hipLaunchKernelGGL((attn_part<T, 128, false>), g, t, 0, st, pv, hv, a);
+    else
+        hipLaunchKernelGGL((attn_part<T, 256, false>), g, t, 0, st, pv, hv, a);
+}
+
 static bool attn_launch(const PoolView &pv, const HeadsView &hv, int dtype, int layer, const float *q,
                         const float *gate, const int *seq, const int *pos, int n, int max_len, float *out, void *work,
                         hipStream_t st) {
-    const dim3 grid(n, hv.H);
+    PagedArgs a;
+    a.q = q, a.gate = gate, a.seq = seq, a.pos = pos, a.out = out, a.n = n, a.layer = layer;
+    a.part = (float *)work;
+    a.ml = (float2 *)(a.part + 2 * (size_t)kAttnBlocks * kGroup * pv.hd);
+    const int G = hv.H / pv.KH;
+    a.groups = (G + kGroup - 1) / kGroup;
+    a.khv = pv.KH * a.groups;
+    a.shift = 0;
+    while ((1L << a.shift) < pv.page) a.shift++;
+    a.magic = (unsigned)(((1ULL << 32) * ((1ULL << a.shift) - pv.page)) / pv.page + 1);
+    const long cap = (long)pv.max_pages * pv.page, units = ((cap + kKeys - 1) / kKeys) * a.khv * (long)n;
+    const int blocks = (int)(units < kAttnBlocks ? units : kAttnBlocks);
     switch (dtype) {
-    case COLI_HIP_F32:
-        hipLaunchKernelGGL(attn_rows<COLI_HIP_F32>, grid, dim3(64 * kRowWaves), 0, st, pv, hv, layer, q, gate, seq, pos, out);
-        break;
-    case COLI_HIP_F16:
-        hipLaunchKernelGGL(attn_rows<COLI_HIP_F16>, grid, dim3(64 * kRowWaves), 0, st, pv, hv, layer, q, gate, seq, pos, out);
-        break;
-    default:
-        hipLaunchKernelGGL(attn_rows<COLI_HIP_BF16>, grid, dim3(64 * kRowWaves), 0, st, pv, hv, layer, q, gate, seq, pos, out);
+    case COLI_HIP_F32: attn_launch_t<COLI_HIP_F32>(pv, hv, a, blocks, st); break;
+    case COLI_HIP_F16: attn_launch_t<COLI_HIP_F16>(pv, hv, a, blocks, st); break;
+    default: attn_launch_t<COLI_HIP_BF16>(pv, hv, a, blocks, st);
     }
+    if (blocks > 1)
+        hipLaunchKernelGGL(attn_join, dim3(blocks - 1, G < kGroup ? G : kGroup), dim3(kAttnThreads), 0, st, pv, hv, a,
+                           blocks);
     return launched("paged attention launch");
 }
 
@@ -280,7 +632,7 @@ COLI_API int coli_hip_qk_rope_paged(const ColiHipPages *p, const ColiHipHeads *h
 COLI_API size_t coli_hip_attn_paged_work(const ColiHipPages *p, const ColiHipHeads *h) {
     PoolView pv;
     HeadsView hv;
-    return pool_view(p, pv) && heads_view(p, h, hv) ? 256 : 0;
+    return pool_view(p, pv) && heads_view(p, h, hv) ? attn_work(pv) : 0;
 }
 
 COLI_API int coli_hip_attn_paged(const ColiHipPages *p, const ColiHipHeads *h, int layer, const float *d_q,
