@@ -30,10 +30,38 @@ struct PoolView {
     long row_bytes, head_bytes, kv_bytes, layer_bytes, page_bytes;
 };
 
+// ColiHipHeads as the kernels take it.
+struct HeadsView {
+    int H, rot, interleaved;
+    long q_row, q_head, kv_row;
+    float eps, mag, scale;
+    const float *qn, *kn, *freq;
+};
+
+// The last position that row n sees (-1: none), and its sequence (-1: no row).
+__device__ __forceinline__ int row_pos(const PoolView &p, const int *seq, const int *pos, int n, int &s) {
+    s = seq[n];
+    if (s < 0 || s >= p.n_seqs) {
+        if (s != -1) atomicOr(&p.state[kStErr], kPgIndex);
+        s = -1;
+        return -1;
+    }
+    const int len = min(max(p.lens[s], 0), p.max_pages * p.page), at = pos ? pos[n] : len - 1;
+    if (at < len && at >= -1) return at;
+    atomicOr(&p.state[kStErr], at < -1 ? kPgIndex : kPgPos);
+    return at < -1 ? -2 : -3 - len;   // -2: no position; -3 - len: past the end
+}
+
 // false, with a message, when the description is outside what the kernels take (host only)
 bool pool_view(const ColiHipPages *p, PoolView &v);
 // the stream of a call and whether it can run: device usable and current
 bool paged_stream(void *stream, hipStream_t &st);
 bool paged_refuse(const char *why);
+bool paged_launched(const char *what);   // no error of the launches before it
+
+// The attention of n rows (paged_attn.hip) on device pointers, and the bytes of its workspace.
+size_t attn_paged_work(const PoolView &p);
+bool attn_paged(const PoolView &p, const HeadsView &h, int dtype, int layer, const float *q, const float *gate,
+                const int *seq, const int *pos, int n, int max_len, float *out, void *work, hipStream_t st);
 
 }  // namespace coli

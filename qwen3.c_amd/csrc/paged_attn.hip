@@ -1,0 +1,727 @@
+// paged_attn.hip - attention of one query row per token over the pages of its sequence.
+//
+//   o = sum_t softmax_t(scale q . k_t) v_t over t <= pos, times sigmoid(gate)
+//
+// in one pass over K and V with a running maximum m and sum l per head (scores in units of
+// log 2: the scale and log2 e are folded into q).
+//
+// A wave takes a tile of keys of one kv head with up to 16 of its query heads, and both
+// products run on the matrix cores straight from the lanes' own loads:
+//   scores [key][head] = K q^T: a lane's 16-byte pieces of key row l % 16 are the A operand; lane
+//     l ends up with keys 4 (l / 16) + i of column l % 16.
+//   out [row][column] += P V: the lane's own weights are the A operand (any order of the keys
+//     does, the same on both sides), and B wants the lane's keys of one column: a lane loads
+//     8 values of each of its keys' V rows and regroups them by column with one byte permute
+//     per two values.  No transpose goes through LDS.
+// Pages of f32 use v_mfma_f32_16x16x4_f32 as they are, 16 keys a tile.  Pages of 16 bits, 32
+// keys a tile, use the 16-bit products (K and V are exact there), with q and the weights as a sum
+// of pieces: 3 of bf16 (24 bits) or 2 of f16 (22 bits; q scaled by a power of two per head, the
+// weights by 2^kUp).  The pieces are further rows of the same products: GS (4, 8 or 16) rows per
+// piece, so 8 heads in f16 and 4 in bf16 cost one product, and the 16 rows are seldom idle.
+// The f32 products they replace took 8 times the matrix cycles of one 16-bit product.
+//   A piece times an infinity can be NaN where the product is infinite: when a result is not
+// finite, the block computes its part again in plain fp32 (slow_part), which gives what the
+// formula gives.
+//
+// Work: a unit is kKeys keys (a tile per wave) of a kv head; the units of all rows in one line
+// are cut into equal shares, one per block, whatever the lengths are.  A (row, kv head) that a
+// border cuts goes through the workspace, and attn_join joins its parts.
+#include "paged.h"
+
+#include <math.h>
+
+namespace coli {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kGroup = 16;   // kGroup: heads a wave takes
+constexpr int kMaxBlocks = 1024;
+constexpr int kWindow = 2048;   // keys whose row offsets a block holds in LDS at a time
+constexpr float kLazy = 8.f;    // the maximum moves when a score passes it by 2^8: weights stay below
+constexpr float kLog2e = 1.4426950408889634f;
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+
+// A (row, kv head) cut by the border behind a block: what attn_join needs of it.
+struct Cut {
+    int row, head, heads, parts;   // first query head, heads, parts (0: none; negative: its first part is in slot 2 b)
+};
+
+struct PagedArgs {
+    const float *q, *gate;
+    const int *seq, *pos;
+    float *out, *part;
+    float2 *ml;
+    Cut *cut;
+    int n, layer, groups, khv;   // head groups of kGroup per kv head, khv = KH * groups
+    unsigned magic, shift;       // t / page = (umulhi(t, magic) + t) >> shift, t < 2^31
+};
+
+// The positions that row r sees (a row of no sequence: -1).
+__device__ __forceinline__ int row_count(const PoolView &p, const PagedArgs &a, int r, int &s) {
+    const int at = row_pos(p, a.seq, a.pos, r, s);
+    return s < 0 ? -1 : at < -2 ? -3 - at : at < 0 ? 0 : at + 1;   // past the end: what is held
+}
+template <int kKeys>
+__device__ __forceinline__ int chunks_of(int cnt) {
+    return cnt < 1 ? cnt + 1 : (int)(((unsigned)cnt + kKeys - 1) / kKeys);   // an empty row has one
+}
+
+__device__ __forceinline__ unsigned page_of(const PagedArgs &a, unsigned t) {
+    return (__umulhi(t, a.magic) + t) >> a.shift;
+}
+
+template <int T>
+struct Pieces;
+template <>
+struct Pieces<COLI_HIP_F32> {
+    static constexpr int n = 1, up = 0;
+};
+template <>
+struct Pieces<COLI_HIP_BF16> {
+    static constexpr int n = 3, up = 0;
+};
+template <>
+struct Pieces<COLI_HIP_F16> {
+    static constexpr int n = 2, up = 6;   // weights of 2^6 at the maximum, 2^14 at most: small ones keep their bits
+};
+
+template <int T>
+__device__ __forceinline__ float widen(unsigned word, int half) {
+    if (T == COLI_HIP_F32) return __uint_as_float(word);
+    if (T == COLI_HIP_BF16) return __uint_as_float(half ? word & 0xffff0000u : word << 16);
+    return (float)__builtin_bit_cast(_Float16, (unsigned short)(half ? word >> 16 : word));
+}
+template <int T>
+__device__ __forceinline__ unsigned pack(float x, float y) {   // to nearest, ties to even
+    if (T == COLI_HIP_BF16) {
+        typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(unsigned, v2b{(__bf16)x, (__bf16)y});
+    }
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, v2h{(_Float16)x, (_Float16)y});
+}
+template <int T>
+__device__ __forceinline__ v4f mfma16(v4u x, v4u y, v4f c) {
+    if (T == COLI_HIP_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0, 0);
+}
+
+// The values of lanes l ^ 16 and l ^ 32 beside the lane's own.
+__device__ __forceinline__ float other16(float x) { return __shfl_xor(x, 16); }
+__device__ __forceinline__ float other32(float x) { return __shfl_xor(x, 32); }
+template <int N>   // the value n lanes further in the row of 16
+__device__ __forceinline__ float ror(float x) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x120 + N, 0xf, 0xf, true));
+}
+// the sum over a head's columns (pieces) of a score
+template <int GS>
+__device__ __forceinline__ float sum_pieces(float x) {
+    if (GS <= 8) x += ror<8>(x);
+    if (GS <= 4) x += ror<4>(x);
+    return x;
+}
+
+__device__ __forceinline__ float finish(float o, float l, int cnt, const float *gate, long at) {
+    o = cnt ? o / l : 0.f;
+    return gate ? o / (1.f + expf(-gate[at])) : o;
+}
+
+// A part in plain fp32: keys [from, last) of the row, a key per wave at a time, four columns a
+// lane, head by head.
+template <int T>
+__device__ void slow_part(const PoolView &p, const HeadsView &h, const PagedArgs &a, int r, int s, int kh, long head,
+                          int hn, int cnt, int from, int last, bool whole, long slot, float *s_o, float *s_ml) {
+    constexpr int kUp = Pieces<T>::up;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = 4 * lane;
+    const bool in = d0 < p.hd;
+    const int *row = p.table + (size_t)s * p.max_pages;
+    const char *base = p.data + (size_t)a.layer * p.layer_bytes + (size_t)kh * p.head_bytes;
+    for (int hh = 0; hh < hn; hh++) {
+        float x[4] = {}, o[4] = {}, m = -INFINITY, l = 0.f;
+        if (in)
+            for (int i = 0; i < 4; i++) x[i] = a.q[((long)r * h.H + head + hh) * p.hd + d0 + i] * (h.scale * kLog2e);
+        for (int t = from + wave; t < last; t += kWaves) {
+            const unsigned j = page_of(a, t);
+            const int pg = row[j];
+            if (pg < 0 || pg >= p.n_pages) continue;
+            const char *kr = base + (size_t)pg * p.page_bytes + (size_t)(t - j * p.page) * p.row_bytes;
+            float k[4] = {}, v[4] = {}, dot = 0.f;
+            if (in)
+                for (int i = 0; i < 4; i++) {
+                    const int d = d0 + i, w = T == COLI_HIP_F32 ? d : d / 2;
+                    k[i] = widen<T>(((const unsigned *)kr)[w], d & 1);
+                    v[i] = widen<T>(((const unsigned *)(kr + p.kv_bytes))[w], d & 1);
+                    dot = fmaf(x[i], k[i], dot);
+                }
+            for (int sft = 32; sft; sft >>= 1) dot += __shfl_xor(dot, sft);
+            const float nm = fmaxf(m, dot), f = m == nm ? 1.f : __builtin_amdgcn_exp2f(m - nm);
+            const float w = dot == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(dot - nm + kUp);
+            for (int i = 0; i < 4; i++) o[i] = fmaf(o[i], f, w * v[i]);
+            l = fmaf(l, f, w);
+            m = nm;
+        }
+        __syncthreads();
+        if (in)
+            for (int i = 0; i < 4; i++) s_o[wave * 256 + d0 + i] = o[i];
+        if (lane == 0) s_ml[2 * wave] = m, s_ml[2 * wave + 1] = l;
+        __syncthreads();
+        float M = -INFINITY, L = 0.f, f[kWaves];
+        for (int w = 0; w < kWaves; w++) M = fmaxf(M, s_ml[2 * w]);
+        for (int w = 0; w < kWaves; w++) {
+            f[w] = s_ml[2 * w] == M ? 1.f : __builtin_amdgcn_exp2f(s_ml[2 * w] - M);
+            L += f[w] * s_ml[2 * w + 1];
+        }
+        const int d = threadIdx.x;
+        if (d < p.hd) {
+            float t = 0.f;
+            for (int w = 0; w < kWaves; w++) t += f[w] * s_o[w * 256 + d];
+            if (whole)
+                a.out[((long)r * h.H + head + hh) * p.hd + d] =
+                    finish(t, L, cnt, a.gate, r * h.q_row + (head + hh) * h.q_head + d);
+            else
+                a.part[(slot * kGroup + hh) * p.hd + d] = t;
+        }
+        if (!whole && d == 0) a.ml[slot * kGroup + hh] = make_float2(M, L);
+    }
+    __syncthreads();
+}
+
+// HD: the head dim, or the next of 64, 128, 256 above it (kExact false).  GS: rows of a piece, at
+// least the heads of a group.
+template <int T, int HD, bool kExact, int GS>
+__global__ __launch_bounds__(kThreads, 2) void attn_part(PoolView p, HeadsView h, PagedArgs a) {
+    constexpr bool kWide = T == COLI_HIP_F32;
+    constexpr int kTile = kWide ? 16 : 32, kSub = kTile / 16, kKeys = kWaves * kTile;
+    constexpr int kPieces = Pieces<T>::n, kUp = Pieces<T>::up, kNT = kWide ? 1 : (kPieces * GS + 15) / 16;
+    constexpr int kKE = kWide ? 4 : 8, kKC = HD / (4 * kKE);                       // K: values of a piece, pieces of a lane
+    constexpr int kVE = HD >= 16 * kKE ? kKE : HD / 16, kVS = HD / (16 * kVE);     // V alike
+    constexpr int kVW = kWide ? kVE : kVE / 2, kVK = kTile / 4;                    // words of a V piece, keys of a lane
+    constexpr int kPad = kKeys + kTile;                                            // offsets read past the last key
+    constexpr int kQRow = kWide ? HD + 4 : HD / 2 + 4;                             // words of a q row in LDS
+    __shared__ long s_base[kThreads], s_wave[kWaves];
+    __shared__ int s_cnt[kThreads];
+    __shared__ long s_off[kWindow + kPad];
+    __shared__ __attribute__((aligned(16))) unsigned s_q[kNT * 16 * kQRow];
+    __shared__ float s_inv[kGroup], s_m[kWaves][kGroup], s_l[kWaves][kGroup];
+    __shared__ __attribute__((aligned(16))) float s_o[2][HD / 16 * 256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int G = h.H / p.KH;
+
+    // the units of all rows in one line; s_base[t]: those before the rows of thread t
+    const int per = (a.n + kThreads - 1) / kThreads;
+    long mine = 0, total = 0;
+    for (int i = 0; i < per; i++) {
+        const int r = tid * per + i;
+        int s;
+        const int cnt = r < a.n ? row_count(p, a, r, s) : -1;
+        s_cnt[tid] = cnt;
+        mine += (long)chunks_of<kKeys>(cnt) * a.khv;
+    }
+    long x = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 63) s_wave[wave] = x;
+    if (!kWide)   // rows of q past the last piece stay zero
+        for (int i = kPieces * GS * kQRow + tid; i < kNT * 16 * kQRow; i += kThreads) s_q[i] = 0;
+    __syncthreads();
+    long before = 0;
+    for (int w = 0; w < kWaves; w++) {
+        before += w < wave ? s_wave[w] : 0;
+        total += s_wave[w];
+    }
+    s_base[tid] = before + x - mine;
+    // (total + blocks - 1) / blocks: below 2^53 and a fraction of at least 1 / blocks from a whole number
+    const long share = (long)((double)(total + gridDim.x - 1) / (double)gridDim.x);
+    const long u0 = blockIdx.x * share, end = min(total, u0 + share);
+    Cut cut = {0, 0, 0, 0};
+    __syncthreads();
+    if (u0 >= end) {
+        if (tid == 0) a.cut[blockIdx.x] = cut;
+        return;
+    }
+    int r, lo = 0, hi = kThreads;   // the thread with the last s_base at or before u0
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (s_base[mid] <= u0)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    r = lo * per;
+    long first = s_base[lo];   // units before row r
+
+    for (long u = u0; u < end && r < a.n;) {
+        int s, cnt;
+        if (per == 1) {
+            s = a.seq[r];
+            cnt = s_cnt[r];
+        } else {
+            cnt = row_count(p, a, r, s);
+        }
+        const int nc = chunks_of<kKeys>(cnt);
+        const long xx = u - first;
+        if (xx >= (long)nc * a.khv) {   // this row is done (or has none)
+            first += (long)nc * a.khv;
+            r++;
+            continue;
+        }
+        const int hv = (int)((unsigned)xx / (unsigned)nc), c0 = (int)xx - hv * nc, c1 = (int)min((long)nc, c0 + (end - u));
+        const int kh = hv / a.groups, h0 = (hv - kh * a.groups) * kGroup, hn = min(kGroup, G - h0);
+        const long head = (long)kh * G + h0;   // the first query head
+        const int from = c0 * kKeys, last = min(cnt, c1 * kKeys);
+        const int *row = p.table + (size_t)s * p.max_pages;
+        const long fix = a.layer * p.layer_bytes + kh * p.head_bytes;
+
+        // q in units of log 2, in pieces; a wave takes every fourth head
+        float qx[GS / kWaves][HD / 64];
+#pragma unroll
+        for (int k = 0; k < GS / kWaves; k++)
+#pragma unroll
+            for (int i = 0; i < HD / 64; i++) {
+                const int hh = wave + kWaves * k, d = lane + 64 * i;
+                qx[k][i] = hh < hn && (kExact || d < p.hd) ? a.q[((long)r * h.H + head + hh) * p.hd + d] : 0.f;
+            }
+        // where the keys' rows lie (-1: no such key)
+        auto fill = [&](int w0, int nk) {
+            for (int i = tid; i < nk + kPad; i += kThreads) {
+                long off = -1;
+                if (i < nk) {
+                    const unsigned t = w0 + i, j = page_of(a, t);
+                    const int pg = row[j];
+                    if (pg >= 0 && pg < p.n_pages)
+                        off = pg * p.page_bytes + fix + (long)(t - j * p.page) * p.row_bytes;
+                    else
+                        atomicOr(&p.state[kStErr], kPgPage);
+                }
+                s_off[i] = off;
+            }
+        };
+        fill(from, min(last - from, kWindow));
+#pragma unroll
+        for (int k = 0; k < GS / kWaves; k++) {
+            const int hh = wave + kWaves * k;
+            float big = 0.f;
+#pragma unroll
+            for (int i = 0; i < HD / 64; i++) {
+                qx[k][i] *= h.scale * kLog2e;
+                big = fmaxf(big, fabsf(qx[k][i]));
+            }
+            if (T == COLI_HIP_F16) {   // the largest of a head in [2^14, 2^15)
+#pragma unroll
+                for (int o = 32; o; o >>= 1) big = fmaxf(big, __shfl_xor(big, o));
+                const int e = big > 0.f && big < INFINITY ? min(14 - ilogbf(big), 100) : 0;
+#pragma unroll
+                for (int i = 0; i < HD / 64; i++) qx[k][i] = ldexpf(qx[k][i], e);
+                if (lane == 0) s_inv[hh] = ldexpf(1.f, -e);
+            }
+#pragma unroll
+            for (int i = 0; i < HD / 64; i++) {
+                const int d = lane + 64 * i;
+                if (kWide) {
+                    s_q[hh * kQRow + d] = __float_as_uint(qx[k][i]);
+                } else {
+                    float rest = qx[k][i];
+#pragma unroll
+                    for (int e = 0; e < kPieces; e++) {
+                        const unsigned w = pack<T>(rest, 0.f);
+                        ((unsigned short *)s_q)[(e * GS + hh) * 2 * kQRow + d] = (unsigned short)w;
+                        rest -= widen<T>(w, 0);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const float inv = T == COLI_HIP_F16 ? s_inv[c % GS] : 1.f;
+
+        v4f acc[kVS][kVE];
+#pragma unroll
+        for (int i = 0; i < kVS; i++)
+#pragma unroll
+            for (int e = 0; e < kVE; e++) acc[i][e] = v4f{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+
+        for (int w0 = from; w0 < last; w0 += kWindow) {
+            const int nk = min(last - w0, kWindow);
+            if (w0 != from) {
+                __syncthreads();
+                fill(w0, nk);
+                __syncthreads();
+            }
+            // a row that is always there, for the loads of keys that are not
+            const long hot = max(s_off[0], 0L);
+            v4u kb[kSub][kKC];
+            unsigned vb[kVK][kVS][kVW];
+            unsigned vm[kSub], vm_next[kSub];
+            auto load_k = [&](int i0) {
+#pragma unroll
+                for (int t = 0; t < kSub; t++) {
+                    const long o = s_off[i0 + 16 * t + c];
+                    vm_next[t] = (unsigned)__ballot(o >= 0) & 0xffffu;
+                    const v4u *k = (const v4u *)(p.data + (o >= 0 ? o : hot));
+#pragma unroll
+                    for (int i = 0; i < kKC; i++) {
+                        const int at = 4 * i + g;
+                        kb[t][i] = k[kExact || at * kKE < p.hd ? at : 0];
+                    }
+                }
+            };
+            auto load_v = [&](int i0) {
+#pragma unroll
+                for (int j = 0; j < kVK; j++) {
+                    const long o = s_off[i0 + 16 * (j / 4) + 4 * g + j % 4];
+                    const char *v = p.data + p.kv_bytes + (o >= 0 ? o : hot);
+#pragma unroll
+                    for (int i = 0; i < kVS; i++) {
+                        int d = (16 * i + c) * kVE;
+                        if (!kExact && d >= p.hd) d = 0;
+                        if (kVW == 4)
+                            *(uint4 *)vb[j][i] = *(const uint4 *)(v + d * (kWide ? 4 : 2));
+                        else
+                            *(uint2 *)vb[j][i] = *(const uint2 *)(v + d * (kWide ? 4 : 2));
+                    }
+                }
+            };
+            load_k(wave * kTile);
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(wave * kTile);
+            __builtin_amdgcn_sched_barrier(0);
+            for (int i0 = wave * kTile; i0 < nk; i0 += kKeys) {
+                unsigned all = 0xffffu;
+#pragma unroll
+                for (int t = 0; t < kSub; t++) all &= vm[t] = vm_next[t];
+                // scores
+                v4f sc[kSub];
+                {
+                    v4f d[kSub][kWide ? 2 : kNT];
+#pragma unroll
+                    for (int t = 0; t < kSub; t++)
+#pragma unroll
+                        for (int e = 0; e < (kWide ? 2 : kNT); e++) d[t][e] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < kKC; i++) {
+                        if constexpr (kWide) {
+                            const v4u qv = *(const v4u *)&s_q[c * kQRow + (4 * i + g) * 4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                d[0][e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                    __uint_as_float(kb[0][i][e]), __uint_as_float(qv[e]), d[0][e & 1], 0, 0, 0);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < kNT; e++) {
+                                const v4u qv = *(const v4u *)&s_q[(16 * e + c) * kQRow + (4 * i + g) * 4];
+#pragma unroll
+                                for (int t = 0; t < kSub; t++) d[t][e] = mfma16<T>(kb[t][i], qv, d[t][e]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < kSub; t++) {
+                        sc[t] = d[t][0];
+#pragma unroll
+                        for (int e = 1; e < (kWide ? 2 : kNT); e++) sc[t] += d[t][e];
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                load_k(i0 + kKeys);
+                __builtin_amdgcn_sched_barrier(0);
+                float mt = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < kSub; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (!kWide) sc[t][i] = sum_pieces<GS>(sc[t][i]);
+                        if (T == COLI_HIP_F16) sc[t][i] *= inv;
+                    }
+                if (all != 0xffffu) {   // keys that are not there: no score, and nothing of V
+#pragma unroll
+                    for (int j = 0; j < kVK; j++) {
+                        if (vm[j / 4] >> (4 * g + j % 4) & 1) continue;
+                        sc[j / 4][j % 4] = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < kVS; i++)
+#pragma unroll
+                            for (int w = 0; w < kVW; w++) vb[j][i][w] = 0;
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < kSub; t++) mt = fmaxf(mt, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])));
+                mt = fmaxf(mt, other16(mt));
+                mt = fmaxf(mt, other32(mt));
+                if (__any(mt > m + kLazy)) {
+                    const float nm = fmaxf(m, mt), f = m == nm ? 1.f : __builtin_amdgcn_exp2f(m - nm);
+                    l *= f;
+                    m = nm;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float fr = __shfl(f, 4 * g + i);
+#pragma unroll
+                        for (int t = 0; t < kVS; t++)
+#pragma unroll
+                            for (int e = 0; e < kVE; e++) acc[t][e][i] *= fr;
+                    }
+                }
+                float w[kVK];
+#pragma unroll
+                for (int j = 0; j < kVK; j++) {
+                    const float x = sc[j / 4][j % 4];
+                    w[j] = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - m + kUp);
+                    l += w[j];
+                }
+                // out += P V
+                if constexpr (kWide) {
+#pragma unroll
+                    for (int j = 0; j < kVK; j++)
+#pragma unroll
+                        for (int i = 0; i < kVS; i++)
+#pragma unroll
+                            for (int e = 0; e < kVE; e++)
+                                acc[i][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], __uint_as_float(vb[j][i][e]),
+                                                                                 acc[i][e], 0, 0, 0);
+                } else {
+                    v4u pw[kPieces], pa[kNT];
+#pragma unroll
+                    for (int e = 0; e < kPieces; e++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            pw[e][j] = pack<T>(w[2 * j], w[2 * j + 1]);
+                            w[2 * j] -= widen<T>(pw[e][j], 0);
+                            w[2 * j + 1] -= widen<T>(pw[e][j], 1);
+                        }
+#pragma unroll
+                    for (int e = 0; e < kNT; e++) {   // row c of product e is piece (16 e + c) / GS
+                        pa[e] = v4u{0, 0, 0, 0};
+#pragma unroll
+                        for (int k = 0; k < kPieces; k++) {
+                            if ((k + 1) * GS <= 16 * e || k * GS >= 16 * e + 16) continue;
+                            const bool is = (16 * e + c) / GS == k;
+#pragma unroll
+                            for (int j = 0; j < 4; j++) pa[e][j] = is ? pw[k][j] : pa[e][j];
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < kVS; i++)
+#pragma unroll
+                        for (int x = 0; x < kVE; x++) {
+                            v4u b;
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                b[j] = __builtin_amdgcn_perm(vb[2 * j + 1][i][x / 2], vb[2 * j][i][x / 2],
+                                                             x & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                            for (int e = 0; e < kNT; e++) acc[i][x] = mfma16<T>(pa[e], b, acc[i][x]);
+                        }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                load_v(i0 + kKeys);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+
+        const bool whole = c0 == 0 && c1 == nc;
+        const long slot = 2L * blockIdx.x + (u == u0 ? 0 : 1);
+        // the four waves' parts under one maximum
+        l += other16(l);
+        l += other32(l);
+        if (g == 0) {
+            s_m[wave][c] = m;
+            s_l[wave][c] = l;
+        }
+        float z = l;
+        if (!kWide) {
+#pragma unroll
+            for (int t = 0; t < kVS; t++)
+#pragma unroll
+                for (int e = 0; e < kVE; e++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) z = fmaf(acc[t][e][i], 0.f, z);
+        }
+        if (__syncthreads_or(!kWide && !(fabsf(z) < INFINITY))) {
+            slow_part<T>(p, h, a, r, s, kh, head, hn, cnt, from, last, whole, slot, s_o[0], &s_m[0][0]);
+        } else {
+            float M[4], f[4], L[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int hh = (4 * g + i) % GS;
+                M[i] = fmaxf(fmaxf(s_m[0][hh], s_m[1][hh]), fmaxf(s_m[2][hh], s_m[3][hh]));
+                L[i] = 0.f;
+                for (int w = 0; w < kWaves; w++) {
+                    const float mw = s_m[w][hh], fw = mw == M[i] ? 1.f : __builtin_amdgcn_exp2f(mw - M[i]);
+                    L[i] += s_l[w][hh] * fw;
+                    if (w == wave) f[i] = fw;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < kVS; t++)
+#pragma unroll
+                for (int e = 0; e < kVE; e++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[t][e][i] *= f[i];
+#pragma unroll
+            for (int step = 2; step; step >>= 1) {
+                if (wave >= step && wave < 2 * step) {
+#pragma unroll
+                    for (int t = 0; t < kVS; t++)
+#pragma unroll
+                        for (int e = 0; e < kVE; e++) *(v4f *)&s_o[wave - step][((t * kVE + e) * 64 + lane) * 4] = acc[t][e];
+                }
+                __syncthreads();
+                if (wave < step) {
+#pragma unroll
+                    for (int t = 0; t < kVS; t++)
+#pragma unroll
+                        for (int e = 0; e < kVE; e++) acc[t][e] += *(const v4f *)&s_o[wave][((t * kVE + e) * 64 + lane) * 4];
+                }
+                __syncthreads();
+            }
+            if (wave == 0) {
+                // rows of one head's pieces: 8 apart (lanes 32 apart) or 4 (16)
+#pragma unroll
+                for (int t = 0; t < kVS; t++)
+#pragma unroll
+                    for (int e = 0; e < kVE; e++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            if (!kWide && GS <= 8) acc[t][e][i] += other32(acc[t][e][i]);
+                            if (!kWide && GS <= 4) acc[t][e][i] += other16(acc[t][e][i]);
+                        }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int hh = 4 * g + i;
+                    if (hh >= hn) continue;   // hn <= GS
+                    float *dst = whole ? a.out + ((long)r * h.H + head + hh) * p.hd : a.part + (slot * kGroup + hh) * p.hd;
+                    const long gat = r * h.q_row + (head + hh) * h.q_head;
+                    if (!whole && c == 0) a.ml[slot * kGroup + hh] = make_float2(M[i], L[i]);
+#pragma unroll
+                    for (int t = 0; t < kVS; t++) {
+                        const int d0 = (16 * t + c) * kVE;
+                        if (!kExact && d0 >= p.hd) continue;
+                        float o[kVE];
+#pragma unroll
+                        for (int e = 0; e < kVE; e++)
+                            o[e] = whole ? finish(acc[t][e][i], L[i], cnt, a.gate, gat + d0 + e) : acc[t][e][i];
+#pragma unroll
+                        for (int e = 0; e < kVE; e += 4) *(float4 *)(dst + d0 + e) = *(const float4 *)(o + e);
+                    }
+                }
+            }
+        }
+        if (c0 == 0 && c1 < nc) {   // goes on in the next blocks
+            const long parts = (long)((double)(u + nc - 1) / (double)share) - blockIdx.x + 1;
+            cut = Cut{r, (int)head, hn, u == u0 ? -(int)parts : (int)parts};
+        }
+        u += c1 - c0;
+    }
+    if (tid == 0) a.cut[blockIdx.x] = cut;
+}
+
+// Block (b, hh): head hh of the (row, kv head) that begins in block b of attn_part and goes on
+// behind it.
+__global__ __launch_bounds__(kThreads) void attn_join(PoolView p, HeadsView h, PagedArgs a) {
+    __shared__ float s_w[kMaxBlocks], s_red[kWaves], s_o[kThreads];
+    const Cut cut = a.cut[blockIdx.x];
+    const int hh = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (!cut.parts || hh >= cut.heads) return;
+    const int n = abs(cut.parts);
+    const long s0 = 2L * blockIdx.x + (cut.parts < 0 ? 0 : 1);
+    auto at = [&](int k) { return (k ? 2L * (blockIdx.x + k) : s0) * kGroup + hh; };
+    float m = -INFINITY, l = 0.f;
+    for (int k = tid; k < n; k += kThreads) m = fmaxf(m, a.ml[at(k)].x);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (lane == 0) s_red[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    __syncthreads();
+    for (int k = tid; k < n; k += kThreads) {
+        const float2 ml = a.ml[at(k)];
+        const float f = ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
+        s_w[k] = f;
+        l += f * ml.y;
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+    if (lane == 0) s_red[wave] = l;
+    __syncthreads();
+    l = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
+    // the threads side by side on the columns; fewer than 256 columns: several on a column's parts
+    const int wide = p.hd <= 64 ? 64 : p.hd <= 128 ? 128 : 256, d = tid % wide, k0 = tid / wide, ks = kThreads / wide;
+    float o = 0.f;
+    if (d < p.hd) {
+#pragma unroll 8
+        for (int k = k0; k < n; k += ks) o = fmaf(s_w[k], a.part[at(k) * p.hd + d], o);
+    }
+    s_o[tid] = o;
+    __syncthreads();
+    if (tid >= p.hd) return;
+    for (int k = 1; k < ks; k++) o += s_o[tid + k * wide];
+    a.out[((long)cut.row * h.H + cut.head + hh) * p.hd + tid] =
+        finish(o, l, 1, a.gate, cut.row * h.q_row + (cut.head + hh) * h.q_head + tid);
+}
+
+static int max_blocks(int hd) { return hd <= 128 ? 1024 : 512; }
+
+size_t attn_paged_work(const PoolView &p) {
+    const size_t b = max_blocks(p.hd);
+    return 2 * b * kGroup * (p.hd * sizeof(float) + sizeof(float2)) + b * sizeof(Cut);
+}
+
+template <int T, int GS>
+static void launch(const PoolView &pv, const HeadsView &hv, const PagedArgs &a, int blocks, hipStream_t st) {
+    const dim3 g(blocks), t(kThreads);
+    switch (pv.hd) {
+    case 64: hipLaunchKernelGGL((attn_part<T, 64, true, GS>), g, t, 0, st, pv, hv, a); return;
+    case 128: hipLaunchKernelGGL((attn_part<T, 128, true, GS>), g, t, 0, st, pv, hv, a); return;
+    case 256: hipLaunchKernelGGL((attn_part<T, 256, true, GS>), g, t, 0, st, pv, hv, a); return;
+    }
+    if (pv.hd < 64)
+        hipLaunchKernelGGL((attn_part<T, 64, false, GS>), g, t, 0, st, pv, hv, a);
+    else if (pv.hd < 128)
+        hipLaunchKernelGGL((attn_part<T, 128, false, GS>), g, t, 0, st, pv, hv, a);
+    else
+        hipLaunchKernelGGL((attn_part<T, 256, false, GS>), g, t, 0, st, pv, hv, a);
+}
+
+template <int T>
+static void launch_heads(const PoolView &pv, const HeadsView &hv, const PagedArgs &a, int blocks, hipStream_t st) {
+    const int G = hv.H / pv.KH;
+    if (G <= 4)
+        launch<T, 4>(pv, hv, a, blocks, st);
+    else if (G <= 8)
+        launch<T, 8>(pv, hv, a, blocks, st);
+    else
+        launch<T, 16>(pv, hv, a, blocks, st);
+}
+
+bool attn_paged(const PoolView &pv, const HeadsView &hv, int dtype, int layer, const float *q, const float *gate,
+                const int *seq, const int *pos, int n, int max_len, float *out, void *work, hipStream_t st) {
+    const int most = max_blocks(pv.hd), G = hv.H / pv.KH, keys = dtype == COLI_HIP_F32 ? 64 : 128;
+    PagedArgs a;
+    a.q = q, a.gate = gate, a.seq = seq, a.pos = pos, a.out = out, a.n = n, a.layer = layer;
+    a.part = (float *)work;
+    a.ml = (float2 *)(a.part + 2 * (size_t)most * kGroup * pv.hd);
+    a.cut = (Cut *)(a.ml + 2 * (size_t)most * kGroup);
+    a.groups = (G + kGroup - 1) / kGroup;
+    a.khv = pv.KH * a.groups;
+    a.shift = 0;
+    while ((1L << a.shift) < pv.page) a.shift++;
+    a.magic = (unsigned)(((1ULL << 32) * ((1ULL << a.shift) - pv.page)) / pv.page + 1);
+    const long cap = (long)pv.max_pages * pv.page, len = max_len > 0 && max_len < cap ? max_len : cap;
+    const long units = ((len + keys - 1) / keys) * a.khv * (long)n;
+    const int blocks = (int)(units < most ? units : most);
+    switch (dtype) {
+    case COLI_HIP_F32: launch<COLI_HIP_F32, 16>(pv, hv, a, blocks, st); break;
+    case COLI_HIP_F16: launch_heads<COLI_HIP_F16>(pv, hv, a, blocks, st); break;
+    default: launch_heads<COLI_HIP_BF16>(pv, hv, a, blocks, st);
+    }
+    if (blocks > 1)
+        hipLaunchKernelGGL(attn_join, dim3(blocks, G < kGroup ? G : kGroup), dim3(kThreads), 0, st, pv, hv, a);
+    return paged_launched("paged attention launch");
+}
+
+}  // namespace coli

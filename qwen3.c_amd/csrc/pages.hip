@@ -57,7 +57,7 @@ bool paged_stream(void *stream_, hipStream_t &st) {
     return true;
 }
 
-static bool launched(const char *what) {
+bool paged_launched(const char *what) {
     const hipError_t e = hipGetLastError();
     return e == hipSuccess || fail(what, e);
 }
@@ -417,7 +417,7 @@ COLI_API int coli_hip_pages_init(const ColiHipPages *p, void *stream_) {
     const size_t most = (size_t)v.n_seqs * v.max_pages, all = most > (size_t)v.n_pages ? most : v.n_pages;
     const unsigned grid = (unsigned)(all / 256 + 1 < 2048 ? all / 256 + 1 : 2048);
     hipLaunchKernelGGL(pages_clear, dim3(grid), dim3(256), 0, st, v);
-    return launched("pages init") ? 1 : 0;
+    return paged_launched("pages init") ? 1 : 0;
 }
 
 static bool take_args(const ColiHipPages *p, PoolView &v, const void *seq, int n) {
@@ -432,7 +432,7 @@ COLI_API int coli_hip_pages_append(const ColiHipPages *p, const int *d_seq, cons
     if (!take_args(p, v, d_seq, n) || !paged_stream(stream_, st)) return 0;
     if (!n) return 1;
     hipLaunchKernelGGL(pages_take, dim3(1), dim3(kPgThreads), 0, st, v, d_seq, d_seq, d_count, n, (int)kTakeAppend);
-    return launched("pages append") ? 1 : 0;
+    return paged_launched("pages append") ? 1 : 0;
 }
 
 COLI_API int coli_hip_pages_fork(const ColiHipPages *p, const int *d_src, const int *d_dst, int n, int share,
@@ -449,7 +449,7 @@ COLI_API int coli_hip_pages_fork(const ColiHipPages *p, const int *d_src, const 
     y = y < 1 ? 1 : y > 2048 ? 2048 : y;
     hipLaunchKernelGGL(pages_fork_copy, dim3(n, (unsigned)y), dim3(kCopyThreads), 0, st, v, d_src, d_dst, share ? 1 : 0,
                        pieces);
-    return launched("pages fork") ? 1 : 0;
+    return paged_launched("pages fork") ? 1 : 0;
 }
 
 COLI_API int coli_hip_pages_free(const ColiHipPages *p, const int *d_seq, int n, void *stream_) {
@@ -458,7 +458,7 @@ COLI_API int coli_hip_pages_free(const ColiHipPages *p, const int *d_seq, int n,
     if (!take_args(p, v, d_seq, n) || !paged_stream(stream_, st)) return 0;
     if (!n) return 1;
     hipLaunchKernelGGL(pages_drop, dim3(n), dim3(kCopyThreads), 0, st, v, d_seq);
-    return launched("pages free") ? 1 : 0;
+    return paged_launched("pages free") ? 1 : 0;
 }
 
 COLI_API int coli_hip_pages_compact(const ColiHipPages *p, void *stream_) {
@@ -467,7 +467,7 @@ COLI_API int coli_hip_pages_compact(const ColiHipPages *p, void *stream_) {
     if (!pool_view(p, v) || !paged_stream(stream_, st)) return 0;
     hipLaunchKernelGGL(pages_plan, dim3(1), dim3(kPgThreads), 0, st, v);
     hipLaunchKernelGGL(pages_move, dim3(8 * n_cu()), dim3(kCopyThreads), 0, st, v, pieces_of(v));
-    return launched("pages compact") ? 1 : 0;
+    return paged_launched("pages compact") ? 1 : 0;
 }
 
 COLI_API int coli_hip_pages_status(const ColiHipPages *p, int *n_free, int *errors, void *stream_) {
