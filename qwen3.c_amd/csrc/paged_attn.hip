@@ -34,19 +34,26 @@ namespace coli {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kGroup = 16;   // kGroup: heads a wave takes
 constexpr int kMaxBlocks = 1024;
-constexpr int kWindow = 2048;   // keys whose row offsets a block holds in LDS at a time
+constexpr int kWindow = 1024;   // keys whose row offsets a block holds in LDS at a time
 constexpr float kLazy = 8.f;    // the maximum moves when a score passes it by 2^8: weights stay below
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
 
 // A (row, kv head) cut by the border behind a block: what attn_join needs of it.
 struct Cut {
     int row, head, heads, parts;   // first query head, heads, parts (0: none; negative: its first part is in slot 2 b)
 };
+
+// Keys of a wave's tile, and blocks that fit a CU by their registers.
+constexpr int tile_of(int T, int HD) { return T == COLI_HIP_F32 || HD == 256 ? 16 : 32; }
+constexpr int resident(int T, int HD) { return HD == 256 ? (T == COLI_HIP_F32 ? 1 : 2) : HD == 128 ? 2 : 3; }
 
 struct PagedArgs {
     const float *q, *gate;
@@ -102,11 +109,18 @@ __device__ __forceinline__ unsigned pack(float x, float y) {   // to nearest, ti
     typedef _Float16 v2h __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(unsigned, v2h{(_Float16)x, (_Float16)y});
 }
+// 16-bit products of 8 (4) values a lane: 32 (16) of the summed index
 template <int T>
 __device__ __forceinline__ v4f mfma16(v4u x, v4u y, v4f c) {
     if (T == COLI_HIP_BF16)
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, y), c, 0, 0, 0);
+}
+template <int T>
+__device__ __forceinline__ v4f mfma16(v2u x, v2u y, v4f c) {
+    if (T == COLI_HIP_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(v4s, x), __builtin_bit_cast(v4s, y), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(v4h, x), __builtin_bit_cast(v4h, y), c, 0, 0, 0);
 }
 
 // The values of lanes l ^ 16 and l ^ 32 beside the lane's own.
@@ -125,8 +139,8 @@ __device__ __forceinline__ float sum_pieces(float x) {
 }
 
 __device__ __forceinline__ float finish(float o, float l, int cnt, const float *gate, long at) {
-    o = cnt ? o / l : 0.f;
-    return gate ? o / (1.f + expf(-gate[at])) : o;
+    const float d = gate ? l * (1.f + expf(-gate[at])) : l;
+    return cnt ? o / d : 0.f;
 }
 
 // A part in plain fp32: keys [from, last) of the row, a key per wave at a time, four columns a
@@ -192,32 +206,36 @@ __device__ void slow_part(const PoolView &p, const HeadsView &h, const PagedArgs
 // HD: the head dim, or the next of 64, 128, 256 above it (kExact false).  GS: rows of a piece, at
 // least the heads of a group.
 template <int T, int HD, bool kExact, int GS>
-__global__ __launch_bounds__(kThreads, 2) void attn_part(PoolView p, HeadsView h, PagedArgs a) {
+__global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView p, HeadsView h, PagedArgs a) {
     constexpr bool kWide = T == COLI_HIP_F32;
-    constexpr int kTile = kWide ? 16 : 32, kSub = kTile / 16, kKeys = kWaves * kTile;
+    constexpr int kTile = tile_of(T, HD), kSub = kTile / 16, kKeys = kWaves * kTile;
     constexpr int kPieces = Pieces<T>::n, kUp = Pieces<T>::up, kNT = kWide ? 1 : (kPieces * GS + 15) / 16;
     constexpr int kKE = kWide ? 4 : 8, kKC = HD / (4 * kKE);                       // K: values of a piece, pieces of a lane
     constexpr int kVE = HD >= 16 * kKE ? kKE : HD / 16, kVS = HD / (16 * kVE);     // V alike
     constexpr int kVW = kWide ? kVE : kVE / 2, kVK = kTile / 4;                    // words of a V piece, keys of a lane
     constexpr int kPad = kKeys + kTile;                                            // offsets read past the last key
     constexpr int kQRow = kWide ? HD + 4 : HD / 2 + 4;                             // words of a q row in LDS
-    __shared__ long s_base[kThreads], s_wave[kWaves];
-    __shared__ int s_cnt[kThreads];
-    __shared__ long s_off[kWindow + kPad];
-    __shared__ __attribute__((aligned(16))) unsigned s_q[kNT * 16 * kQRow];
+    constexpr int kQWords = kNT * 16 * kQRow, kOffWords = 2 * (kWindow + kPad), kSum = HD * 16;
+    // q and the offsets of the keys' rows, then the waves' sums
+    __shared__ __attribute__((aligned(16))) unsigned s_mem[kQWords + kOffWords > 2 * kSum ? kQWords + kOffWords : 2 * kSum];
+    __shared__ int s_cnt[kThreads], s_seq[kThreads], s_row;
+    __shared__ long s_wave[kWaves], s_first;
     __shared__ float s_inv[kGroup], s_m[kWaves][kGroup], s_l[kWaves][kGroup];
-    __shared__ __attribute__((aligned(16))) float s_o[2][HD / 16 * 256];
+    unsigned *const s_q = s_mem;
+    long *const s_off = (long *)(s_mem + kQWords);
+    float *const s_o = (float *)s_mem;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     const int G = h.H / p.KH;
 
-    // the units of all rows in one line; s_base[t]: those before the rows of thread t
+    // the units of all rows in one line: a thread has `per` rows
     const int per = (a.n + kThreads - 1) / kThreads;
     long mine = 0, total = 0;
     for (int i = 0; i < per; i++) {
         const int r = tid * per + i;
-        int s;
+        int s = -1;
         const int cnt = r < a.n ? row_count(p, a, r, s) : -1;
         s_cnt[tid] = cnt;
+        s_seq[tid] = s;
         mine += (long)chunks_of<kKeys>(cnt) * a.khv;
     }
     long x = mine;
@@ -227,39 +245,40 @@ __global__ __launch_bounds__(kThreads, 2) void attn_part(PoolView p, HeadsView h
         if (lane >= o) x += y;
     }
     if (lane == 63) s_wave[wave] = x;
-    if (!kWide)   // rows of q past the last piece stay zero
-        for (int i = kPieces * GS * kQRow + tid; i < kNT * 16 * kQRow; i += kThreads) s_q[i] = 0;
     __syncthreads();
-    long before = 0;
+    long before = x - mine;
     for (int w = 0; w < kWaves; w++) {
         before += w < wave ? s_wave[w] : 0;
         total += s_wave[w];
     }
-    s_base[tid] = before + x - mine;
     // (total + blocks - 1) / blocks: below 2^53 and a fraction of at least 1 / blocks from a whole number
     const long share = (long)((double)(total + gridDim.x - 1) / (double)gridDim.x);
     const long u0 = blockIdx.x * share, end = min(total, u0 + share);
-    Cut cut = {0, 0, 0, 0};
-    __syncthreads();
     if (u0 >= end) {
-        if (tid == 0) a.cut[blockIdx.x] = cut;
+        if (tid == 0) a.cut[blockIdx.x] = Cut{0, 0, 0, 0};
         return;
     }
-    int r, lo = 0, hi = kThreads;   // the thread with the last s_base at or before u0
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (s_base[mid] <= u0)
-            lo = mid;
-        else
-            hi = mid;
+    if (before <= u0 && u0 < before + mine) {   // unit u0 is in a row of this thread's
+        int r = tid * per;
+        for (int i = 1; i < per; i++) {
+            int s;
+            const long k = (long)chunks_of<kKeys>(row_count(p, a, r, s)) * a.khv;
+            if (before + k > u0) break;
+            before += k;
+            r++;
+        }
+        s_row = r;
+        s_first = before;
     }
-    r = lo * per;
-    long first = s_base[lo];   // units before row r
+    __syncthreads();
+    int r = s_row;
+    long first = s_first;   // units before row r
+    Cut cut = {0, 0, 0, 0};
 
     for (long u = u0; u < end && r < a.n;) {
         int s, cnt;
         if (per == 1) {
-            s = a.seq[r];
+            s = s_seq[r];
             cnt = s_cnt[r];
         } else {
             cnt = row_count(p, a, r, s);
@@ -287,6 +306,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_part(PoolView p, HeadsView h
                 const int hh = wave + kWaves * k, d = lane + 64 * i;
                 qx[k][i] = hh < hn && (kExact || d < p.hd) ? a.q[((long)r * h.H + head + hh) * p.hd + d] : 0.f;
             }
+        if (!kWide)   // rows of q past the last piece
+            for (int i = kPieces * GS * kQRow + tid; i < kQWords; i += kThreads) s_q[i] = 0;
         // where the keys' rows lie (-1: no such key)
         auto fill = [&](int w0, int nk) {
             for (int i = tid; i < nk + kPad; i += kThreads) {
@@ -484,33 +505,36 @@ __global__ __launch_bounds__(kThreads, 2) void attn_part(PoolView p, HeadsView h
                                 acc[i][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], __uint_as_float(vb[j][i][e]),
                                                                                  acc[i][e], 0, 0, 0);
                 } else {
-                    v4u pw[kPieces], pa[kNT];
+                    constexpr int kPW = kVK / 2;   // words of a lane's weights
+                    typedef unsigned vp __attribute__((ext_vector_type(kPW)));
+                    vp pw[kPieces], pa[kNT];
 #pragma unroll
                     for (int e = 0; e < kPieces; e++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
+                        for (int j = 0; j < kPW; j++) {
                             pw[e][j] = pack<T>(w[2 * j], w[2 * j + 1]);
                             w[2 * j] -= widen<T>(pw[e][j], 0);
                             w[2 * j + 1] -= widen<T>(pw[e][j], 1);
                         }
 #pragma unroll
                     for (int e = 0; e < kNT; e++) {   // row c of product e is piece (16 e + c) / GS
-                        pa[e] = v4u{0, 0, 0, 0};
+#pragma unroll
+                        for (int j = 0; j < kPW; j++) pa[e][j] = 0;
 #pragma unroll
                         for (int k = 0; k < kPieces; k++) {
                             if ((k + 1) * GS <= 16 * e || k * GS >= 16 * e + 16) continue;
                             const bool is = (16 * e + c) / GS == k;
 #pragma unroll
-                            for (int j = 0; j < 4; j++) pa[e][j] = is ? pw[k][j] : pa[e][j];
+                            for (int j = 0; j < kPW; j++) pa[e][j] = is ? pw[k][j] : pa[e][j];
                         }
                     }
 #pragma unroll
                     for (int i = 0; i < kVS; i++)
 #pragma unroll
                         for (int x = 0; x < kVE; x++) {
-                            v4u b;
+                            vp b;
 #pragma unroll
-                            for (int j = 0; j < 4; j++)
+                            for (int j = 0; j < kPW; j++)
                                 b[j] = __builtin_amdgcn_perm(vb[2 * j + 1][i][x / 2], vb[2 * j][i][x / 2],
                                                              x & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
@@ -542,74 +566,61 @@ __global__ __launch_bounds__(kThreads, 2) void attn_part(PoolView p, HeadsView h
                     for (int i = 0; i < 4; i++) z = fmaf(acc[t][e][i], 0.f, z);
         }
         if (__syncthreads_or(!kWide && !(fabsf(z) < INFINITY))) {
-            slow_part<T>(p, h, a, r, s, kh, head, hn, cnt, from, last, whole, slot, s_o[0], &s_m[0][0]);
+            slow_part<T>(p, h, a, r, s, kh, head, hn, cnt, from, last, whole, slot, s_o, &s_m[0][0]);
         } else {
-            float M[4], f[4], L[4];
+            const float M = fmaxf(fmaxf(s_m[0][c], s_m[1][c]), fmaxf(s_m[2][c], s_m[3][c]));
+            const float f = m == M ? 1.f : __builtin_amdgcn_exp2f(m - M);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int hh = (4 * g + i) % GS;
-                M[i] = fmaxf(fmaxf(s_m[0][hh], s_m[1][hh]), fmaxf(s_m[2][hh], s_m[3][hh]));
-                L[i] = 0.f;
-                for (int w = 0; w < kWaves; w++) {
-                    const float mw = s_m[w][hh], fw = mw == M[i] ? 1.f : __builtin_amdgcn_exp2f(mw - M[i]);
-                    L[i] += s_l[w][hh] * fw;
-                    if (w == wave) f[i] = fw;
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < kVS; t++)
-#pragma unroll
-                for (int e = 0; e < kVE; e++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[t][e][i] *= f[i];
-#pragma unroll
-            for (int step = 2; step; step >>= 1) {
-                if (wave >= step && wave < 2 * step) {
-#pragma unroll
-                    for (int t = 0; t < kVS; t++)
-#pragma unroll
-                        for (int e = 0; e < kVE; e++) *(v4f *)&s_o[wave - step][((t * kVE + e) * 64 + lane) * 4] = acc[t][e];
-                }
-                __syncthreads();
-                if (wave < step) {
-#pragma unroll
-                    for (int t = 0; t < kVS; t++)
-#pragma unroll
-                        for (int e = 0; e < kVE; e++) acc[t][e] += *(const v4f *)&s_o[wave][((t * kVE + e) * 64 + lane) * 4];
-                }
-                __syncthreads();
-            }
-            if (wave == 0) {
-                // rows of one head's pieces: 8 apart (lanes 32 apart) or 4 (16)
+                const float fr = __shfl(f, 4 * g + i);   // of row 4 g + i
 #pragma unroll
                 for (int t = 0; t < kVS; t++)
 #pragma unroll
-                    for (int e = 0; e < kVE; e++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            if (!kWide && GS <= 8) acc[t][e][i] += other32(acc[t][e][i]);
-                            if (!kWide && GS <= 4) acc[t][e][i] += other16(acc[t][e][i]);
-                        }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int hh = 4 * g + i;
-                    if (hh >= hn) continue;   // hn <= GS
-                    float *dst = whole ? a.out + ((long)r * h.H + head + hh) * p.hd : a.part + (slot * kGroup + hh) * p.hd;
-                    const long gat = r * h.q_row + (head + hh) * h.q_head;
-                    if (!whole && c == 0) a.ml[slot * kGroup + hh] = make_float2(M[i], L[i]);
-#pragma unroll
-                    for (int t = 0; t < kVS; t++) {
-                        const int d0 = (16 * t + c) * kVE;
-                        if (!kExact && d0 >= p.hd) continue;
-                        float o[kVE];
-#pragma unroll
-                        for (int e = 0; e < kVE; e++)
-                            o[e] = whole ? finish(acc[t][e][i], L[i], cnt, a.gate, gat + d0 + e) : acc[t][e][i];
-#pragma unroll
-                        for (int e = 0; e < kVE; e += 4) *(float4 *)(dst + d0 + e) = *(const float4 *)(o + e);
-                    }
-                }
+                    for (int e = 0; e < kVE; e++) acc[t][e][i] *= fr;
             }
+            // waves 2 and 3 into 0 and 1, whose sums the threads then add and write
+            float *so = s_o + (wave & 1) * kSum + 4 * lane;
+            if (wave >= 2) {
+#pragma unroll
+                for (int t = 0; t < kVS * kVE; t++) *(v4f *)(so + 256 * t) = acc[t / kVE][t % kVE];
+            }
+            __syncthreads();
+            if (wave < 2) {
+#pragma unroll
+                for (int t = 0; t < kVS * kVE; t++) *(v4f *)(so + 256 * t) = acc[t / kVE][t % kVE] + *(v4f *)(so + 256 * t);
+            }
+            __syncthreads();
+            // a thread: head hh's kVE columns from d0.  Rows of one head's pieces are GS apart.
+            for (int i = tid; i < hn * kVS * 16; i += kThreads) {
+                const int hh = i / 16 % hn, t = i / 16 / hn, d0 = (16 * t + (i & 15)) * kVE;
+                if (!kExact && d0 >= p.hd) continue;
+                float mw[kWaves], M = -INFINITY, L = 0.f, o[kVE];
+#pragma unroll
+                for (int w = 0; w < kWaves; w++) M = fmaxf(M, mw[w] = s_m[w][hh]);
+#pragma unroll
+                for (int w = 0; w < kWaves; w++) L += s_l[w][hh] * (mw[w] == M ? 1.f : __builtin_amdgcn_exp2f(mw[w] - M));
+#pragma unroll
+                for (int e = 0; e < kVE; e++) o[e] = 0.f;
+#pragma unroll
+                for (int k = 0; k < (kWide ? 1 : 16 / GS); k++) {
+                    const int row = hh + k * GS;
+                    const float *at = s_o + 256 * kVE * t + (row / 4 * 16 + (i & 15)) * 4 + row % 4;
+#pragma unroll
+                    for (int e = 0; e < kVE; e++) o[e] += at[256 * e] + at[kSum + 256 * e];
+                }
+                float *dst = a.part + (slot * kGroup + hh) * p.hd + d0;
+                if (whole) {
+                    dst = a.out + ((long)r * h.H + head + hh) * p.hd + d0;
+                    const long gat = r * h.q_row + (head + hh) * h.q_head + d0;
+#pragma unroll
+                    for (int e = 0; e < kVE; e++) o[e] = finish(o[e], L, cnt, a.gate, gat + e);
+                } else if (d0 == 0) {
+                    a.ml[slot * kGroup + hh] = make_float2(M, L);
+                }
+#pragma unroll
+                for (int e = 0; e < kVE; e += 4) *(float4 *)(dst + e) = *(const float4 *)(o + e);
+            }
+            __syncthreads();   // the sums' place is the next part's q
         }
         if (c0 == 0 && c1 < nc) {   // goes on in the next blocks
             const long parts = (long)((double)(u + nc - 1) / (double)share) - blockIdx.x + 1;
@@ -664,10 +675,11 @@ __global__ __launch_bounds__(kThreads) void attn_join(PoolView p, HeadsView h, P
         finish(o, l, 1, a.gate, cut.row * h.q_row + (cut.head + hh) * h.q_head + tid);
 }
 
-static int max_blocks(int hd) { return hd <= 128 ? 1024 : 512; }
+// Blocks of a launch: all of them resident, so that equal shares end together.
+static int max_blocks(int T, int hd) { return 256 * resident(T, hd <= 64 ? 64 : hd <= 128 ? 128 : 256); }
 
 size_t attn_paged_work(const PoolView &p) {
-    const size_t b = max_blocks(p.hd);
+    const size_t b = max_blocks(p.es == 4 ? COLI_HIP_F32 : COLI_HIP_F16, p.hd);
     return 2 * b * kGroup * (p.hd * sizeof(float) + sizeof(float2)) + b * sizeof(Cut);
 }
 
@@ -700,7 +712,8 @@ static void launch_heads(const PoolView &pv, const HeadsView &hv, const PagedArg
 
 bool attn_paged(const PoolView &pv, const HeadsView &hv, int dtype, int layer, const float *q, const float *gate,
                 const int *seq, const int *pos, int n, int max_len, float *out, void *work, hipStream_t st) {
-    const int most = max_blocks(pv.hd), G = hv.H / pv.KH, keys = dtype == COLI_HIP_F32 ? 64 : 128;
+    const int most = max_blocks(dtype, pv.hd), G = hv.H / pv.KH;
+    const int keys = kWaves * tile_of(dtype, pv.hd <= 64 ? 64 : pv.hd <= 128 ? 128 : 256);
     PagedArgs a;
     a.q = q, a.gate = gate, a.seq = seq, a.pos = pos, a.out = out, a.n = n, a.layer = layer;
     a.part = (float *)work;
