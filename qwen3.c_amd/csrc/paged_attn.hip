@@ -23,9 +23,11 @@
 // finite, the block computes its part again in plain fp32 (slow_part), which gives what the
 // formula gives.
 //
-// Work: a unit is kKeys keys (a tile per wave) of a kv head; the units of all rows in one line
-// are cut into equal shares, one per block, whatever the lengths are.  A (row, kv head) that a
-// border cuts goes through the workspace, and attn_join joins its parts.
+// Work: a unit is kKeys keys (a tile per wave) of a kv head, 64 KB or so; a (row, kv head) counts
+// kSetup units more, about what its q, row offsets and sums cost beside the keys (200 ragged rows
+// of 45 to 2900 keys: SETUPTIMES).  The units of all rows in one line are cut into equal shares, one
+// per block, whatever the lengths are.  A (row, kv head) that a border cuts goes through the
+// workspace, and attn_join joins its parts.
 #include "paged.h"
 
 #include <math.h>
@@ -53,7 +55,7 @@ struct Cut {
 
 // Keys of a wave's tile, and blocks that fit a CU by their registers.
 constexpr int tile_of(int T, int HD) { return T == COLI_HIP_F32 || HD == 256 ? 16 : 32; }
-constexpr int resident(int T, int HD) { return HD == 256 ? (T == COLI_HIP_F32 ? 1 : 2) : HD == 128 ? 2 : 3; }
+constexpr int resident(int T, int HD) { return HD == 256 ? (T == COLI_HIP_F32 ? 1 : 2) : HD == 128 ? 2 : 4; }
 
 struct PagedArgs {
     const float *q, *gate;
@@ -71,8 +73,19 @@ __device__ __forceinline__ int row_count(const PoolView &p, const PagedArgs &a, 
     return s < 0 ? -1 : at < -2 ? -3 - at : at < 0 ? 0 : at + 1;   // past the end: what is held
 }
 template <int kKeys>
-__device__ __forceinline__ int chunks_of(int cnt) {
-    return cnt < 1 ? cnt + 1 : (int)(((unsigned)cnt + kKeys - 1) / kKeys);   // an empty row has one
+__device__ __forceinline__ int chunks_of(int cnt) {   // an empty row has one
+    return cnt < 1 ? 1 : (int)(((unsigned)cnt + kKeys - 1) / kKeys);
+}
+// the units of a row per kv head
+template <int kKeys, int kSetup>
+__device__ __forceinline__ int units_of(int cnt) {
+    return cnt < 0 ? 0 : chunks_of<kKeys>(cnt) + kSetup;
+}
+
+// A value that every lane holds alike, in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long uniform(long x) {
+    return (long)(((unsigned long)(unsigned)uniform((int)(x >> 32)) << 32) | (unsigned)uniform((int)x));
 }
 
 __device__ __forceinline__ unsigned page_of(const PagedArgs &a, unsigned t) {
@@ -213,6 +226,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
     constexpr int kKE = kWide ? 4 : 8, kKC = HD / (4 * kKE);                       // K: values of a piece, pieces of a lane
     constexpr int kVE = HD >= 16 * kKE ? kKE : HD / 16, kVS = HD / (16 * kVE);     // V alike
     constexpr int kVW = kWide ? kVE : kVE / 2, kVK = kTile / 4;                    // words of a V piece, keys of a lane
+    constexpr int kUnit = kKeys * HD * (kWide ? 8 : 4), kSetup = kUnit >= 65536 ? 1 : 65536 / kUnit;
     constexpr int kPad = kKeys + kTile;                                            // offsets read past the last key
     constexpr int kQRow = kWide ? HD + 4 : HD / 2 + 4;                             // words of a q row in LDS
     constexpr int kQWords = kNT * 16 * kQRow, kOffWords = 2 * (kWindow + kPad), kSum = HD * 16;
@@ -224,7 +238,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
     unsigned *const s_q = s_mem;
     long *const s_off = (long *)(s_mem + kQWords);
     float *const s_o = (float *)s_mem;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 15, g = lane >> 4;
     const int G = h.H / p.KH;
 
     // the units of all rows in one line: a thread has `per` rows
@@ -236,7 +250,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         const int cnt = r < a.n ? row_count(p, a, r, s) : -1;
         s_cnt[tid] = cnt;
         s_seq[tid] = s;
-        mine += (long)chunks_of<kKeys>(cnt) * a.khv;
+        mine += (long)units_of<kKeys, kSetup>(cnt) * a.khv;
     }
     long x = mine;
 #pragma unroll
@@ -251,8 +265,9 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         before += w < wave ? s_wave[w] : 0;
         total += s_wave[w];
     }
+    total = uniform(total);
     // (total + blocks - 1) / blocks: below 2^53 and a fraction of at least 1 / blocks from a whole number
-    const long share = (long)((double)(total + gridDim.x - 1) / (double)gridDim.x);
+    const long share = uniform((long)((double)(total + gridDim.x - 1) / (double)gridDim.x));
     const long u0 = blockIdx.x * share, end = min(total, u0 + share);
     if (u0 >= end) {
         if (tid == 0) a.cut[blockIdx.x] = Cut{0, 0, 0, 0};
@@ -262,7 +277,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         int r = tid * per;
         for (int i = 1; i < per; i++) {
             int s;
-            const long k = (long)chunks_of<kKeys>(row_count(p, a, r, s)) * a.khv;
+            const long k = (long)units_of<kKeys, kSetup>(row_count(p, a, r, s)) * a.khv;
             if (before + k > u0) break;
             before += k;
             r++;
@@ -271,9 +286,10 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         s_first = before;
     }
     __syncthreads();
-    int r = s_row;
-    long first = s_first;   // units before row r
+    int r = uniform(s_row);
+    long first = uniform(s_first);   // units before row r
     Cut cut = {0, 0, 0, 0};
+    int done = 0;   // whether the block has had a part before
 
     for (long u = u0; u < end && r < a.n;) {
         int s, cnt;
@@ -283,15 +299,20 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         } else {
             cnt = row_count(p, a, r, s);
         }
-        const int nc = chunks_of<kKeys>(cnt);
+        s = uniform(s);
+        cnt = uniform(cnt);
+        const int nc = chunks_of<kKeys>(cnt), nu = units_of<kKeys, kSetup>(cnt);
         const long xx = u - first;
-        if (xx >= (long)nc * a.khv) {   // this row is done (or has none)
-            first += (long)nc * a.khv;
+        if (xx >= (long)nu * a.khv) {   // this row is done (or has none)
+            first += (long)nu * a.khv;
             r++;
             continue;
         }
-        const int hv = (int)((unsigned)xx / (unsigned)nc), c0 = (int)xx - hv * nc, c1 = (int)min((long)nc, c0 + (end - u));
-        const int kh = hv / a.groups, h0 = (hv - kh * a.groups) * kGroup, hn = min(kGroup, G - h0);
+        const int hv = uniform((int)((unsigned)xx / (unsigned)nu)), x0 = (int)xx - hv * nu;
+        const int x1 = (int)min((long)nu, x0 + (end - u)), c0 = max(x0 - kSetup, 0), c1 = x1 - kSetup;
+        u += x1 - x0;
+        if (c1 <= c0) continue;   // the keys are the next block's
+        const int kh = uniform(hv / a.groups), h0 = (hv - kh * a.groups) * kGroup, hn = min(kGroup, G - h0);
         const long head = (long)kh * G + h0;   // the first query head
         const int from = c0 * kKeys, last = min(cnt, c1 * kKeys);
         const int *row = p.table + (size_t)s * p.max_pages;
@@ -375,7 +396,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
                 __syncthreads();
             }
             // a row that is always there, for the loads of keys that are not
-            const long hot = max(s_off[0], 0L);
+            const long hot = uniform(max(s_off[0], 0L));
             v4u kb[kSub][kKC];
             unsigned vb[kVK][kVS][kVW];
             unsigned vm[kSub], vm_next[kSub];
@@ -548,7 +569,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         }
 
         const bool whole = c0 == 0 && c1 == nc;
-        const long slot = 2L * blockIdx.x + (u == u0 ? 0 : 1);
+        const long slot = 2L * blockIdx.x + done;
         // the four waves' parts under one maximum
         l += other16(l);
         l += other32(l);
@@ -622,11 +643,11 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
             }
             __syncthreads();   // the sums' place is the next part's q
         }
-        if (c0 == 0 && c1 < nc) {   // goes on in the next blocks
-            const long parts = (long)((double)(u + nc - 1) / (double)share) - blockIdx.x + 1;
-            cut = Cut{r, (int)head, hn, u == u0 ? -(int)parts : (int)parts};
+        if (c0 == 0 && c1 < nc) {   // goes on in the next blocks; u is behind its unit c1
+            const int parts = (int)((double)(u + (nc - c1) - 1) / (double)share) - (int)blockIdx.x + 1;
+            cut = Cut{r, (int)head, hn, done ? parts : -parts};
         }
-        u += c1 - c0;
+        done = 1;
     }
     if (tid == 0) a.cut[blockIdx.x] = cut;
 }
@@ -634,7 +655,8 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
 // Block (b, hh): head hh of the (row, kv head) that begins in block b of attn_part and goes on
 // behind it.
 __global__ __launch_bounds__(kThreads) void attn_join(PoolView p, HeadsView h, PagedArgs a) {
-    __shared__ float s_w[kMaxBlocks], s_red[kWaves], s_o[kThreads];
+    __shared__ float s_w[kMaxBlocks], s_red[kWaves];
+    __shared__ v4f s_o[kThreads];
     const Cut cut = a.cut[blockIdx.x];
     const int hh = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (!cut.parts || hh >= cut.heads) return;
@@ -660,19 +682,20 @@ __global__ __launch_bounds__(kThreads) void attn_join(PoolView p, HeadsView h, P
     if (lane == 0) s_red[wave] = l;
     __syncthreads();
     l = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
-    // the threads side by side on the columns; fewer than 256 columns: several on a column's parts
-    const int wide = p.hd <= 64 ? 64 : p.hd <= 128 ? 128 : 256, d = tid % wide, k0 = tid / wide, ks = kThreads / wide;
-    float o = 0.f;
+    // a thread: four columns of every ks-th part
+    const int wide = p.hd <= 64 ? 16 : p.hd <= 128 ? 32 : 64, d = tid % wide * 4, k0 = tid / wide, ks = kThreads / wide;
+    v4f o = {0.f, 0.f, 0.f, 0.f};
     if (d < p.hd) {
 #pragma unroll 8
-        for (int k = k0; k < n; k += ks) o = fmaf(s_w[k], a.part[at(k) * p.hd + d], o);
+        for (int k = k0; k < n; k += ks) o += s_w[k] * *(const v4f *)(a.part + at(k) * p.hd + d);
     }
     s_o[tid] = o;
     __syncthreads();
-    if (tid >= p.hd) return;
+    if (k0 || d >= p.hd) return;
     for (int k = 1; k < ks; k++) o += s_o[tid + k * wide];
-    a.out[((long)cut.row * h.H + cut.head + hh) * p.hd + tid] =
-        finish(o, l, 1, a.gate, cut.row * h.q_row + (cut.head + hh) * h.q_head + tid);
+    const long gat = cut.row * h.q_row + (cut.head + hh) * h.q_head + d;
+    for (int i = 0; i < 4; i++) o[i] = finish(o[i], l, 1, a.gate, gat + i);
+    *(v4f *)(a.out + ((long)cut.row * h.H + cut.head + hh) * p.hd + d) = o;
 }
 
 // Blocks of a launch: all of them resident, so that equal shares end together.
@@ -725,7 +748,7 @@ bool attn_paged(const PoolView &pv, const HeadsView &hv, int dtype, int layer, c
     while ((1L << a.shift) < pv.page) a.shift++;
     a.magic = (unsigned)(((1ULL << 32) * ((1ULL << a.shift) - pv.page)) / pv.page + 1);
     const long cap = (long)pv.max_pages * pv.page, len = max_len > 0 && max_len < cap ? max_len : cap;
-    const long units = ((len + keys - 1) / keys) * a.khv * (long)n;
+    const long units = ((len + keys - 1) / keys) * a.khv * (long)n;   // blocks beyond these would cut setups only
     const int blocks = (int)(units < most ? units : most);
     switch (dtype) {
     case COLI_HIP_F32: launch<COLI_HIP_F32, 16>(pv, hv, a, blocks, st); break;
