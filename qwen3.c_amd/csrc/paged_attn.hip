@@ -48,9 +48,11 @@ typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
 
-// A (row, kv head) cut by the border behind a block: what attn_join needs of it.
+// A (row, kv head) that a border cuts: what attn_join needs of it.  Parts k > 0 are in slots
+// 2 (block + k).
 struct Cut {
-    int row, head, heads, parts;   // first query head, heads, parts (0: none; negative: its first part is in slot 2 b)
+    int row, head, heads, parts;   // first query head, heads, parts (0: not cut)
+    int block, slot;               // of its first part
 };
 
 // Keys of a wave's tile, and blocks that fit a CU by their registers.
@@ -63,6 +65,7 @@ struct PagedArgs {
     float *out, *part;
     float2 *ml;
     Cut *cut;
+    int by_row;                  // cuts are listed by (row, kv head), else by the block they begin in
     int n, layer, groups, khv;   // head groups of kGroup per kv head, khv = KH * groups
     unsigned magic, shift;       // t / page = (umulhi(t, magic) + t) >> shift, t < 2^31
 };
@@ -250,6 +253,8 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         const int cnt = r < a.n ? row_count(p, a, r, s) : -1;
         s_cnt[tid] = cnt;
         s_seq[tid] = s;
+        if (a.by_row && !blockIdx.x && r < a.n && cnt < 0)   // no block has this row
+            for (int k = 0; k < a.khv; k++) a.cut[r * a.khv + k].parts = 0;
         mine += (long)units_of<kKeys, kSetup>(cnt) * a.khv;
     }
     long x = mine;
@@ -270,7 +275,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
     const long share = uniform((long)((double)(total + gridDim.x - 1) / (double)gridDim.x));
     const long u0 = blockIdx.x * share, end = min(total, u0 + share);
     if (u0 >= end) {
-        if (tid == 0) a.cut[blockIdx.x] = Cut{0, 0, 0, 0};
+        if (tid == 0 && !a.by_row) a.cut[blockIdx.x].parts = 0;
         return;
     }
     if (before <= u0 && u0 < before + mine) {   // unit u0 is in a row of this thread's
@@ -288,7 +293,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
     __syncthreads();
     int r = uniform(s_row);
     long first = uniform(s_first);   // units before row r
-    Cut cut = {0, 0, 0, 0};
+    Cut cut = {};
     int done = 0;   // whether the block has had a part before
 
     for (long u = u0; u < end && r < a.n;) {
@@ -643,28 +648,43 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
             }
             __syncthreads();   // the sums' place is the next part's q
         }
-        if (c0 == 0 && c1 < nc) {   // goes on in the next blocks; u is behind its unit c1
-            const int parts = (int)((double)(u + (nc - c1) - 1) / (double)share) - (int)blockIdx.x + 1;
-            cut = Cut{r, (int)head, hn, done ? parts : -parts};
+        if (c0 == 0) {   // u is behind its unit c1
+            cut = Cut{};
+            if (c1 < nc) {
+                const int parts = (int)((double)(u + (nc - c1) - 1) / (double)share) - (int)blockIdx.x + 1;
+                cut = Cut{r, (int)head, hn, parts, (int)blockIdx.x, (int)slot};
+            }
+            if (a.by_row && tid == 0) a.cut[r * a.khv + hv] = cut;
         }
         done = 1;
     }
-    if (tid == 0) a.cut[blockIdx.x] = cut;
+    if (tid == 0 && !a.by_row) a.cut[blockIdx.x] = cut;   // only the last part can go on
 }
 
-// Block (b, hh): head hh of the (row, kv head) that begins in block b of attn_part and goes on
-// behind it.
-__global__ __launch_bounds__(kThreads) void attn_join(PoolView p, HeadsView h, PagedArgs a) {
+// Block (i, hh, z): columns z * cols.. of head hh of cut i.  A thread has four columns of every
+// ks-th part; the first kAhead parts are on their way while the weights are found.
+constexpr int kAhead = 8;
+__global__ __launch_bounds__(kThreads) void attn_join(PoolView p, HeadsView h, PagedArgs a, int cols) {
     __shared__ float s_w[kMaxBlocks], s_red[kWaves];
     __shared__ v4f s_o[kThreads];
     const Cut cut = a.cut[blockIdx.x];
-    const int hh = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (!cut.parts || hh >= cut.heads) return;
-    const int n = abs(cut.parts);
-    const long s0 = 2L * blockIdx.x + (cut.parts < 0 ? 0 : 1);
-    auto at = [&](int k) { return (k ? 2L * (blockIdx.x + k) : s0) * kGroup + hh; };
+    const int hh = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = cut.parts;
+    if (!n || hh >= cut.heads) return;
+    const int wide = cols / 4, d = blockIdx.z * cols + tid % wide * 4, k0 = tid / wide, ks = kThreads / wide;
+    const bool in = d < p.hd;
+    auto at = [&](int k) { return (k ? 2L * (cut.block + k) : (long)cut.slot) * kGroup + hh; };
+    v4f x[kAhead], o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+        const int k = k0 + j * ks;
+        x[j] = k < n && in ? *(const v4f *)(a.part + at(k) * p.hd + d) : o;
+    }
     float m = -INFINITY, l = 0.f;
-    for (int k = tid; k < n; k += kThreads) m = fmaxf(m, a.ml[at(k)].x);
+    for (int k = tid; k < n; k += kThreads) {
+        const float2 ml = a.ml[at(k)];
+        m = fmaxf(m, ml.x);
+        s_w[k] = ml.x;
+    }
 #pragma unroll
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     if (lane == 0) s_red[wave] = m;
@@ -672,26 +692,27 @@ __global__ __launch_bounds__(kThreads) void attn_join(PoolView p, HeadsView h, P
     m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
     __syncthreads();
     for (int k = tid; k < n; k += kThreads) {
-        const float2 ml = a.ml[at(k)];
-        const float f = ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
+        const float f = s_w[k] == m ? 1.f : __builtin_amdgcn_exp2f(s_w[k] - m);
         s_w[k] = f;
-        l += f * ml.y;
+        l += f * a.ml[at(k)].y;
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
     if (lane == 0) s_red[wave] = l;
     __syncthreads();
     l = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
-    // a thread: four columns of every ks-th part
-    const int wide = p.hd <= 64 ? 16 : p.hd <= 128 ? 32 : 64, d = tid % wide * 4, k0 = tid / wide, ks = kThreads / wide;
-    v4f o = {0.f, 0.f, 0.f, 0.f};
-    if (d < p.hd) {
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+        const int k = k0 + j * ks;
+        if (k < n) o += s_w[k] * x[j];
+    }
+    if (in) {
 #pragma unroll 8
-        for (int k = k0; k < n; k += ks) o += s_w[k] * *(const v4f *)(a.part + at(k) * p.hd + d);
+        for (int k = k0 + kAhead * ks; k < n; k += ks) o += s_w[k] * *(const v4f *)(a.part + at(k) * p.hd + d);
     }
     s_o[tid] = o;
     __syncthreads();
-    if (k0 || d >= p.hd) return;
+    if (k0 || !in) return;
     for (int k = 1; k < ks; k++) o += s_o[tid + k * wide];
     const long gat = cut.row * h.q_row + (cut.head + hh) * h.q_head + d;
     for (int i = 0; i < 4; i++) o[i] = finish(o[i], l, 1, a.gate, gat + i);
@@ -750,13 +771,18 @@ bool attn_paged(const PoolView &pv, const HeadsView &hv, int dtype, int layer, c
     const long cap = (long)pv.max_pages * pv.page, len = max_len > 0 && max_len < cap ? max_len : cap;
     const long units = ((len + keys - 1) / keys) * a.khv * (long)n;   // blocks beyond these would cut setups only
     const int blocks = (int)(units < most ? units : most);
+    a.by_row = n * (long)a.khv <= blocks;
     switch (dtype) {
     case COLI_HIP_F32: launch<COLI_HIP_F32, 16>(pv, hv, a, blocks, st); break;
     case COLI_HIP_F16: launch_heads<COLI_HIP_F16>(pv, hv, a, blocks, st); break;
     default: launch_heads<COLI_HIP_BF16>(pv, hv, a, blocks, st);
     }
-    if (blocks > 1)
-        hipLaunchKernelGGL(attn_join, dim3(blocks, G < kGroup ? G : kGroup), dim3(kThreads), 0, st, pv, hv, a);
+    if (blocks > 1) {
+        // few cuts: blocks of 64 columns (16 parts at a time); else of a whole head
+        const int cuts = a.by_row ? n * a.khv : blocks, heads = G < kGroup ? G : kGroup;
+        const int cols = cuts * heads <= 512 ? 64 : pv.hd <= 64 ? 64 : pv.hd <= 128 ? 128 : 256;
+        hipLaunchKernelGGL(attn_join, dim3(cuts, heads, (pv.hd + cols - 1) / cols), dim3(kThreads), 0, st, pv, hv, a, cols);
+    }
     return paged_launched("paged attention launch");
 }
 
