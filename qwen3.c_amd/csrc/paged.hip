@@ -49,68 +49,118 @@ struct Val<COLI_HIP_BF16> {
 
 // ---------------------------------------------------------------- norms, rotation, pages
 // y = x rsqrt(mean x^2 + eps) (1 + w), then the first rot columns turned by pos * freq[j].  The
-// angle is taken in 64 bits (24-bit frequencies times positions of up to 31 bits are exact
+// angle is taken in 64 bits (24-bit frequencies times positions of up to 29 bits are exact
 // there) and reduced to a fraction of a turn before it becomes 32 bits.
-// A wave per head row: block (n, j): j < H a query head, then KH key heads, then KH value rows.
-template <int T>
-__global__ __launch_bounds__(64) void qk_rope_rows(PoolView p, HeadsView h, int layer, const float *__restrict__ q,
-                                                   const float *__restrict__ k, const float *__restrict__ v,
-                                                   const int *__restrict__ seq, const int *__restrict__ pos,
-                                                   float *__restrict__ qo) {
+//
+// Bound by its bytes (q in and out, k and v in, the pages' rows out) where there are many rows,
+// by a launch and three dependent loads (sequence, length, page) where there are few.  A row is
+// LP lanes of four columns each, so a wave has 64 / LP rows (query heads, then key heads, then
+// values) at a time and takes more of the same token: the sines and cosines (one pair a lane) and its columns' norm weights
+// are found once.  4005 rows of 32 + 8 heads of 128, all columns turned: ROPETIMES
+constexpr int kRopeWaves = 4;
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v4u4 __attribute__((ext_vector_type(4), aligned(4)));   // rows need not be aligned
+template <int T, int LP>
+__global__ __launch_bounds__(64 * kRopeWaves) void qk_rope_rows(PoolView p, HeadsView h, int layer,
+                                                                const float *__restrict__ q, const float *__restrict__ k,
+                                                                const float *__restrict__ v, const int *__restrict__ seq,
+                                                                const int *__restrict__ pos, float *__restrict__ qo) {
     using D = typename Val<T>::type;
-    __shared__ float s_row[256];
-    const int n = blockIdx.x, j = blockIdx.y, lane = threadIdx.x;
+    typedef D v4d __attribute__((ext_vector_type(4)));
+    constexpr int kRows = 64 / LP;
+    __shared__ __attribute__((aligned(16))) float s_x[kRopeWaves][256];
+    __shared__ float2 s_turn[kRopeWaves][128];
+    const int n = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, sub = lane / LP, d0 = lane % LP * 4;
+    const int rows = h.H + 2 * p.KH, hr = h.rot / 2;
+    const bool in = d0 < p.hd;
+    int j0 = (blockIdx.y * kRopeWaves + wave) * kRows;
+    const int step = gridDim.y * kRopeWaves * kRows;
+    auto source = [&](int j) {
+        return j < h.H ? q + n * h.q_row + j * h.q_head
+                       : (j < h.H + p.KH ? k : v - (long)p.KH * p.hd) + n * h.kv_row + (long)(j - h.H) * p.hd;
+    };
+    auto load = [&](int j) -> v4f {
+        if (!in || j >= rows) return v4f{0.f, 0.f, 0.f, 0.f};
+        return *(const v4u4 *)(source(j) + d0);
+    };
+    v4f x = load(j0 + sub);
+    v4f wq = {0.f, 0.f, 0.f, 0.f}, wk = wq;
+    if (in && h.qn) wq = *(const v4u4 *)(h.qn + d0);
+    if (in && h.kn) wk = *(const v4u4 *)(h.kn + d0);
+    // the frequencies of pairs lane and lane + 64
+    float fr[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) fr[i] = lane + 64 * i < hr ? h.freq[lane + 64 * i] : 0.f;
     int s;
     const int at = row_pos(p, seq, pos, n, s);
     if (s < 0 || at < 0) return;
-    const int pg = p.table[(size_t)s * p.max_pages + at / p.page];
-    if (j >= h.H && (pg < 0 || pg >= p.n_pages)) {
-        if (lane == 0) atomicOr(&p.state[kStErr], kPgPage);
-        return;
-    }
-    const bool isq = j < h.H, isv = j >= h.H + p.KH;
-    const int kh = isv ? j - h.H - p.KH : j - h.H;
-    const float *src = isq ? q + n * h.q_row + j * h.q_head : (isv ? v : k) + n * h.kv_row + (long)kh * p.hd;
-    D *page = (D *)(p.data + (isq ? 0 : (size_t)pg * p.page_bytes + layer * p.layer_bytes + (isv ? p.kv_bytes : 0) +
-                                            kh * p.head_bytes + (at % p.page) * p.row_bytes));
-    if (isv) {
-        for (int d = lane; d < p.hd; d += 64) page[d] = Val<T>::down(src[d]);
-        return;
-    }
-    const float *w = isq ? h.qn : h.kn;
-    float x[4], ss = 0.f;
+    const int pj = at / p.page, slot = at - pj * p.page;
+    const int pg = p.table[(size_t)s * p.max_pages + pj];
+    const bool bad = pg < 0 || pg >= p.n_pages;
+    if (bad && threadIdx.x == 0) atomicOr(&p.state[kStErr], kPgPage);
+    char *page = p.data + (bad ? 0 : (size_t)pg * p.page_bytes) + layer * p.layer_bytes + slot * p.row_bytes;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int d = lane + 64 * i;
-        x[i] = d < p.hd ? src[d] : 0.f;
-        ss += x[i] * x[i];
+    for (int i = 0; i < 2; i++) {
+        if (64 * i >= hr) break;
+        const double t = (double)at * (double)fr[i], c = 0.15915494309189535;   // c + lo = 1 / (2 pi)
+        const double a = fma(t, c, -rint(t * c)) + t * -9.839338337591243e-18;  // a fraction of a turn
+        float sn, cs;
+        sincospif((float)(2.0 * a), &sn, &cs);
+        s_turn[wave][lane + 64 * i] = make_float2(cs * h.mag, sn * h.mag);
     }
-    for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o);
-    const float r = w ? 1.f / sqrtf(ss / p.hd + h.eps) : 1.f;
+    __builtin_amdgcn_wave_barrier();
+    float cs[4], sn[4];
+    bool second[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int d = lane + 64 * i;
-        if (d < p.hd) s_row[d] = w ? x[i] * r * (1.f + w[d]) : x[i];
+    for (int i = 0; i < 4; i++) {   // the column's pair, and which of the two it is
+        const int d = d0 + i;
+        second[i] = h.interleaved ? d & 1 : d >= hr;
+        const float2 t = s_turn[wave][d >= h.rot ? 0 : h.interleaved ? d / 2 : second[i] ? d - hr : d];
+        cs[i] = t.x;
+        sn[i] = second[i] ? t.y : -t.y;   // (u, v) -> (u cos - v sin, v cos + u sin)
     }
-    __syncthreads();
-    const int hr = h.rot / 2;
-    for (int d = lane; d < p.hd; d += 64) {
-        float o = s_row[d];
-        if (d < h.rot) {
-            const int jj = h.interleaved ? d / 2 : d < hr ? d : d - hr;
-            const bool second = h.interleaved ? d & 1 : d >= hr;
-            const float other = s_row[h.interleaved ? d ^ 1 : second ? d - hr : d + hr];
-            const double x = (double)at * (double)h.freq[jj], c = 0.15915494309189535;   // c + lo = 1 / (2 pi)
-            const double a = fma(x, c, -rint(x * c)) + x * -9.839338337591243e-18;   // a fraction of a turn
-            float sn, cs;
-            sincospif((float)(2.0 * a), &sn, &cs);
-            sn *= h.mag, cs *= h.mag;
-            o = second ? o * cs + other * sn : o * cs - other * sn;
+    for (; j0 < rows; j0 += step) {
+        const int j = j0 + sub;
+        const v4f next = load(j + step);
+        const bool isq = j < h.H, isv = j >= h.H + p.KH, live = in && j < rows;
+        float ss = (x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]);
+#pragma unroll
+        for (int o = LP / 2; o; o >>= 1) ss += __shfl_xor(ss, o);
+        const float *w = isq ? h.qn : h.kn;
+        v4f y = x;
+        if (w) {
+            const float r = 1.f / sqrtf(ss / p.hd + h.eps);
+            const v4f wv = isq ? wq : wk;
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[i] = x[i] * r * (1.f + wv[i]);
         }
-        if (isq)
-            qo[((size_t)n * h.H + j) * p.hd + d] = o;
-        else
-            page[d] = Val<T>::down(o);
+        v4f o = y;
+        if (h.interleaved) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (d0 + i < h.rot) o[i] = y[i] * cs[i] + y[i ^ 1] * sn[i];
+        } else if (h.rot) {   // the other half's columns are other lanes' of this wave
+            float *row = s_x[wave] + sub * 4 * LP;
+            *(v4f *)(row + d0) = y;
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int d = d0 + i;
+                if (d < h.rot) o[i] = y[i] * cs[i] + row[second[i] ? d - hr : d + hr] * sn[i];
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        if (isv) o = x;
+        if (live && isq) {
+            *(v4u4 *)(qo + ((size_t)n * h.H + j) * p.hd + d0) = o;
+        } else if (live && !bad) {
+            v4d r;
+#pragma unroll
+            for (int i = 0; i < 4; i++) r[i] = Val<T>::down(o[i]);
+            const int kh = isv ? j - h.H - p.KH : j - h.H;
+            *(v4d *)(page + (isv ? p.kv_bytes : 0) + kh * p.head_bytes + d0 * sizeof(D)) = r;
+        }
+        x = next;
     }
 }
 
@@ -120,18 +170,27 @@ static bool rows_args(const ColiHipPages *p, int layer, int n) {
     return true;
 }
 
+template <int T>
+static void rope_rows(const PoolView &pv, const HeadsView &hv, int layer, const float *q, const float *k, const float *v,
+                      const int *seq, const int *pos, int n, float *qo, hipStream_t st) {
+    const int lp = pv.hd <= 64 ? 16 : pv.hd <= 128 ? 32 : 64, per = kRopeWaves * (64 / lp);
+    // few tokens: a wave per row; many: the waves of one block take a token's rows in turn
+    const long all = (hv.H + 2 * pv.KH + per - 1) / per, want = (2048 + n - 1) / n;
+    const dim3 grid(n, (unsigned)(all < want ? all : want)), t(64 * kRopeWaves);
+    if (lp == 16)
+        hipLaunchKernelGGL((qk_rope_rows<T, 16>), grid, t, 0, st, pv, hv, layer, q, k, v, seq, pos, qo);
+    else if (lp == 32)
+        hipLaunchKernelGGL((qk_rope_rows<T, 32>), grid, t, 0, st, pv, hv, layer, q, k, v, seq, pos, qo);
+    else
+        hipLaunchKernelGGL((qk_rope_rows<T, 64>), grid, t, 0, st, pv, hv, layer, q, k, v, seq, pos, qo);
+}
+
 static bool rope_launch(const PoolView &pv, const HeadsView &hv, int dtype, int layer, const float *q, const float *k,
                         const float *v, const int *seq, const int *pos, int n, float *qo, hipStream_t st) {
-    const dim3 grid(n, hv.H + 2 * pv.KH);
     switch (dtype) {
-    case COLI_HIP_F32:
-        hipLaunchKernelGGL(qk_rope_rows<COLI_HIP_F32>, grid, dim3(64), 0, st, pv, hv, layer, q, k, v, seq, pos, qo);
-        break;
-    case COLI_HIP_F16:
-        hipLaunchKernelGGL(qk_rope_rows<COLI_HIP_F16>, grid, dim3(64), 0, st, pv, hv, layer, q, k, v, seq, pos, qo);
-        break;
-    default:
-        hipLaunchKernelGGL(qk_rope_rows<COLI_HIP_BF16>, grid, dim3(64), 0, st, pv, hv, layer, q, k, v, seq, pos, qo);
+    case COLI_HIP_F32: rope_rows<COLI_HIP_F32>(pv, hv, layer, q, k, v, seq, pos, n, qo, st); break;
+    case COLI_HIP_F16: rope_rows<COLI_HIP_F16>(pv, hv, layer, q, k, v, seq, pos, n, qo, st); break;
+    default: rope_rows<COLI_HIP_BF16>(pv, hv, layer, q, k, v, seq, pos, n, qo, st);
     }
     return paged_launched("qk rope launch");
 }

@@ -46,7 +46,7 @@ bool pool_view(const ColiHipPages *p, PoolView &v) {
     v.kv_bytes = v.head_bytes * p->KH;
     v.layer_bytes = 2 * v.kv_bytes;
     v.page_bytes = v.layer_bytes * p->n_layers;
-    return true;
+    return v.page_bytes < 1L << 34 || paged_refuse("page of 16 GiB or more");
 }
 
 bool paged_stream(void *stream_, hipStream_t &st) {
@@ -104,13 +104,18 @@ enum { kTakeAppend = 0, kTakeShare = 1, kTakeCopy = 2 };
 __global__ __launch_bounds__(kPgThreads) void pages_take(PoolView p, const int *__restrict__ a,
                                                          const int *__restrict__ b, const int *__restrict__ count,
                                                          int n, int mode) {
+    constexpr int kHash = 2 * kPgMaxN;
     __shared__ int s_off[kPgMaxN + 1];
+    __shared__ int s_list[kPgMaxN];   // the new pages, where they are few
+    __shared__ int s_hash[kHash];     // the sequences named so far
     __shared__ int s_wave[kPgThreads / 64];
     __shared__ int s_err;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, words = (p.n_pages + 31) / 32;
+    const unsigned word0 = tid < words ? used_word(p, tid) : ~0u;
     if (tid == 0) s_err = 0;
+    for (int i = tid; i < kHash; i += kPgThreads) s_hash[i] = -1;
     __syncthreads();
-    // what each needs; a mark per sequence finds the ones named twice
+    // what each needs
     int err = 0;
     for (int i = tid; i < n; i += kPgThreads) {
         const int s = b[i], f = mode == kTakeAppend ? s : a[i];
@@ -118,7 +123,13 @@ __global__ __launch_bounds__(kPgThreads) void pages_take(PoolView p, const int *
         if (s < -1 || s >= p.n_seqs || f < -1 || f >= p.n_seqs) {
             err |= kPgIndex;
         } else if (s >= 0 && f >= 0) {
-            p.work[s] = i;
+            unsigned at = (unsigned)s * 2654435761u % kHash;
+            for (;;) {   // ends: twice as many places as sequences
+                const int old = atomicCAS(&s_hash[at], -1, s);
+                if (old == s) err |= kPgTwice;
+                if (old == -1 || old == s) break;
+                at = (at + 1) % kHash;
+            }
             const int len = p.lens[s];
             const long most = (long)p.max_pages * p.page;
             if (len < 0 || len > most) err |= kPgIndex;
@@ -140,14 +151,9 @@ __global__ __launch_bounds__(kPgThreads) void pages_take(PoolView p, const int *
         s_off[i] = need;
     }
     __syncthreads();
-    for (int i = tid; i < n; i += kPgThreads) {
-        const int s = b[i], f = mode == kTakeAppend ? s : a[i];
-        if (s >= 0 && f >= 0 && s < p.n_seqs && f < p.n_seqs && p.work[s] != i) err |= kPgTwice;
-    }
     // free pages, and the need: each thread sums four neighbours (both at most n_pages, or an error)
-    const int words = (p.n_pages + 31) / 32;
-    int nfree = 0, total_free, total = 0;
-    for (int w = tid; w < words; w += kPgThreads) nfree += 32 - __popc(used_word(p, w));
+    int nfree = 32 - __popc(word0), total_free, total = 0;
+    for (int w = tid + kPgThreads; w < words; w += kPgThreads) nfree += 32 - __popc(used_word(p, w));
     block_scan(nfree, s_wave, &total_free);
     int v[kPgMaxN / kPgThreads], mine = 0, full = 0;
 #pragma unroll
@@ -184,10 +190,10 @@ __global__ __launch_bounds__(kPgThreads) void pages_take(PoolView p, const int *
     if (tid == 0) s_off[n] = total;
     __syncthreads();
     // the lowest `total` free pages, in order, into the list
-    int *list = p.work + p.n_seqs;
+    int *list = total <= kPgMaxN ? s_list : p.work;
     for (int w0 = 0, base = 0; base < total && w0 < words; w0 += kPgThreads) {
         const int w = w0 + tid;
-        unsigned fr = w < words ? ~used_word(p, w) : 0u;
+        unsigned fr = !w0 ? ~word0 : w < words ? ~used_word(p, w) : 0u;
         int found;
         int r = base + block_scan(__popc(fr), s_wave, &found);
         unsigned taken = 0;
@@ -237,21 +243,27 @@ __global__ __launch_bounds__(kPgThreads) void pages_take(PoolView p, const int *
 }
 
 // ---------------------------------------------------------------- copying
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
 // The first `held` rows of every head plane of page `from` to page `to`, piece of pieces.
 __device__ __forceinline__ void copy_page(const PoolView &p, int from, int to, int held, int piece, int pieces) {
-    const uint4 *src = (const uint4 *)(p.data + (size_t)from * p.page_bytes);
-    uint4 *dst = (uint4 *)(p.data + (size_t)to * p.page_bytes);
-    const long row16 = p.row_bytes / 16;
-    if (held == p.page) {
-        const long n = p.page_bytes / 16, per = (n + pieces - 1) / pieces;
-        const long end = min(n, (piece + 1) * per);
-        for (long u = piece * per + threadIdx.x; u < end; u += blockDim.x) dst[u] = src[u];
-        return;
+    const v4u *src = (const v4u *)(p.data + (size_t)from * p.page_bytes);
+    v4u *dst = (v4u *)(p.data + (size_t)to * p.page_bytes);
+    // 16-byte units of a plane held, and from plane to plane
+    const unsigned plane = held * (unsigned)(p.row_bytes / 16), stride = (unsigned)(p.head_bytes / 16);
+    const unsigned n = plane * (unsigned)(p.n_layers * 2 * p.KH), per = (n + pieces - 1) / pieces;
+    const unsigned end = min(n, (piece + 1) * per);
+    auto place = [&](unsigned w) { return plane == stride ? w : w / plane * stride + w % plane; };
+    unsigned u = piece * per + threadIdx.x;
+    for (; u + 3 * kCopyThreads < end; u += 4 * kCopyThreads) {   // four loads before the first store
+        v4u x[4];
+        unsigned at[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = src[at[i] = place(u + i * kCopyThreads)];
+#pragma unroll
+        for (int i = 0; i < 4; i++) dst[at[i]] = x[i];
     }
-    const long plane = held * row16, n = plane * p.n_layers * 2 * p.KH, stride = p.head_bytes / 16;
-    const long per = (n + pieces - 1) / pieces, end = min(n, (piece + 1) * per);
-    for (long u = piece * per + threadIdx.x; u < end; u += blockDim.x) {
-        const long at = u / plane * stride + u % plane;
+    for (; u < end; u += kCopyThreads) {
+        const unsigned at = place(u);
         dst[at] = src[at];
     }
 }
@@ -301,12 +313,14 @@ __global__ __launch_bounds__(kCopyThreads) void pages_drop(PoolView p, const int
         if (s != -1 && threadIdx.x == 0) atomicOr(&p.state[kStErr], kPgIndex);
         return;
     }
+    int *row = p.table + (size_t)s * p.max_pages, next = -1;
     if (threadIdx.x == 0) s_len = atomicExch(&p.lens[s], 0);
+    if (threadIdx.x < p.max_pages) next = row[threadIdx.x];
     __syncthreads();
     const int np = min(pages_of(s_len, p.page), p.max_pages);
-    int *row = p.table + (size_t)s * p.max_pages;
     for (int j = threadIdx.x; j < np; j += kCopyThreads) {
-        const int pg = row[j];
+        const int pg = next;
+        if (j + kCopyThreads < np) next = row[j + kCopyThreads];
         row[j] = -1;
         if (pg < 0 || pg >= p.n_pages) {
             atomicOr(&p.state[kStErr], kPgPage);
@@ -327,7 +341,7 @@ __global__ __launch_bounds__(kPgThreads) void pages_plan(PoolView p) {
     for (int w = tid; w < words; w += kPgThreads) n += 32 - __popc(used_word(p, w));
     block_scan(n, s_wave, &live);
     live = p.n_pages - live;
-    int *hole = p.work + p.n_seqs, *mover = hole + (p.n_pages + 1) / 2 + 1, *to = hole + p.n_pages + 4;
+    int *hole = p.work, *mover = hole + (p.n_pages + 1) / 2 + 1, *to = hole + p.n_pages + 4;
     int nh = 0, nm = 0;
     for (int w0 = 0; w0 < words; w0 += kPgThreads) {
         const int w = w0 + tid;
@@ -368,7 +382,7 @@ __global__ __launch_bounds__(kPgThreads) void pages_plan(PoolView p) {
 __global__ __launch_bounds__(kCopyThreads) void pages_move(PoolView p, int pieces) {
     const int moved = p.state[kStMove], live = p.state[kStLive];
     if (!moved) return;
-    const int *hole = p.work + p.n_seqs, *mover = hole + (p.n_pages + 1) / 2 + 1, *to = hole + p.n_pages + 4;
+    const int *hole = p.work, *mover = hole + (p.n_pages + 1) / 2 + 1, *to = hole + p.n_pages + 4;
     const long tasks = (long)moved * pieces;
     for (long t = blockIdx.x; t < tasks; t += gridDim.x) {
         const int k = (int)(t / pieces);
@@ -407,7 +421,7 @@ COLI_API int coli_hip_pages_check(const ColiHipPages *p) {
 }
 
 COLI_API size_t coli_hip_pages_work(const ColiHipPages *p) {
-    return p && p->n_seqs > 0 && p->n_pages > 0 ? (size_t)p->n_seqs + 2 * (size_t)p->n_pages + 64 : 0;
+    return p && p->n_pages > 0 ? 2 * (size_t)p->n_pages + 64 : 0;
 }
 
 COLI_API int coli_hip_pages_init(const ColiHipPages *p, void *stream_) {
