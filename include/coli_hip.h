@@ -316,7 +316,7 @@ int   coli_hip_gdn_chunked(int on);
  *   state [COLI_HIP_PAGES_STATE] error bits and words of the library
  *   work  [coli_hip_pages_work()] ints of scratch, no contents kept between calls
  * All arrays are the caller's device memory; coli_hip_pages_init fills the bookkeeping ones
- * (not data).  hd is a multiple of 8 in 8..256, page 1..4096.
+ * (not data).  hd is a multiple of 8 in 8..256, page 1..4096, max_pages * page at most 2^30.
  * The functions read and change the arrays on the device, in stream order, with no host
  * decision: a decode step (append, then per layer qk_rope and attn) can be captured into a
  * graph.  Calls on one pool that change it (init, append, fork, free, compact, qk_rope) must be
@@ -333,7 +333,7 @@ typedef struct {
     int dtype, n_layers, KH, hd, page, n_pages, n_seqs, max_pages;
 } ColiHipPages;
 /* 1 when the description is one the library takes (host only, no device needed), else 0 with a
- * message.  Every function below checks it as well. */
+ * message.  Every function below checks it as well.  Rows of a call: at most 2^20. */
 int    coli_hip_pages_check(const ColiHipPages *p);
 /* ints that `work` has to hold. */
 size_t coli_hip_pages_work(const ColiHipPages *p);
@@ -393,8 +393,8 @@ int    coli_hip_qk_rope_paged(const ColiHipPages *p, const ColiHipHeads *h, int 
  * (strides q_row, q_head).  d_q is [n][H][hd] as qk_rope leaves it.  A row that sees no position
  * gives 0; a row with sequence -1 is left as it was; one past the end sees what the sequence
  * holds.  max_len: the longest sequence in the call as far as the caller knows (0: unknown); only the split
- * of the work goes by it.  d_work: coli_hip_attn_paged_work() bytes, aligned to 16, zeroed once
- * before its first use and not shared by calls that may run at once. */
+ * of the work goes by it.  d_out and d_work are aligned to 16 bytes;
+ * d_work: coli_hip_attn_paged_work() bytes, not shared by calls that may run at once, no contents kept. */
 size_t coli_hip_attn_paged_work(const ColiHipPages *p, const ColiHipHeads *h);
 int    coli_hip_attn_paged(const ColiHipPages *p, const ColiHipHeads *h, int layer, const float *d_q,
                            const float *d_gate, const int *d_seq, const int *d_pos, int n, int max_len, float *d_out,
@@ -403,7 +403,7 @@ int    coli_hip_attn_paged(const ColiHipPages *p, const ColiHipHeads *h, int lay
  * rows: d_x [n][D] (normed) -> q (| gate where gq_t has 2 H hd rows), k, v -> qk_rope into the
  * pages -> attention -> out_t -> d_out [n][out_t rows].  The positions must have been appended.
  * A row with sequence -1 gives 0.  The strides of h are not used.  Shares the layer blocks'
- * scratch: one stream. */
+ * scratch: one stream, and not one that is being captured. */
 int    coli_hip_gqa_paged(const ColiHipPages *p, const ColiHipHeads *h, int layer, const float *d_x, int D,
                           const ColiVkTensor *gq_t, const ColiVkTensor *gk_t, const ColiVkTensor *gv_t,
                           const ColiVkTensor *out_t, const int *d_seq, const int *d_pos, int n, int max_len,

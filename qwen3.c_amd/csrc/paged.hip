@@ -13,7 +13,7 @@ namespace coli {
 
 static bool heads_view(const ColiHipPages *p, const ColiHipHeads *h, HeadsView &v) {
     if (!h) return paged_refuse("NULL heads");
-    if (h->H < 1 || h->H % p->KH || h->H > 65536) return paged_refuse("query heads not a multiple of the kv heads");
+    if (h->H < 1 || h->H % p->KH || h->H > 4096) return paged_refuse("query heads not a multiple of the kv heads");
     if (h->rot < 0 || h->rot > p->hd || h->rot % 2) return paged_refuse("rotary columns not even, or more than a head");
     if (h->rot && !h->freq) return paged_refuse("NULL inverse frequencies");
     if (h->q_head < p->hd || h->q_row < (h->H - 1) * h->q_head + p->hd || h->kv_row < (int64_t)p->KH * p->hd)
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void qk_rope_rows(PoolView p, Head
 
 static bool rows_args(const ColiHipPages *p, int layer, int n) {
     if (layer < 0 || layer >= p->n_layers) return paged_refuse("layer index");
-    if (n < 0 || n > 1 << 24) return paged_refuse("row count");
+    if (n < 0 || n > 1 << 20) return paged_refuse("row count not in 0..2^20");
     return true;
 }
 
@@ -247,6 +247,7 @@ COLI_API int coli_hip_attn_paged(const ColiHipPages *p, const ColiHipHeads *h, i
     hipStream_t st;
     if (!pool_view(p, pv) || !heads_view(p, h, hv) || !rows_args(p, layer, n)) return 0;
     if (n && (!d_q || !d_seq || !d_out)) return paged_refuse("NULL rows") ? 1 : 0;
+    if ((uintptr_t)d_out % 16) return paged_refuse("attention output not aligned to 16 bytes") ? 1 : 0;
     if (n && (!d_work || (uintptr_t)d_work % 16 || work_bytes < coli_hip_attn_paged_work(p, h)))
         return paged_refuse("attention workspace missing, too small or not aligned to 16 bytes") ? 1 : 0;
     if (!paged_stream(stream_, st)) return 0;
@@ -274,6 +275,9 @@ COLI_API int coli_hip_gqa_paged(const ColiHipPages *p, const ColiHipHeads *h, in
     own.kv_row = (int64_t)KH * hd;
     if (!heads_view(p, &own, hv) || !paged_stream(stream_, st)) return 0;
     if (!n) return 1;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(st, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone)
+        return paged_refuse("the layer block in a captured stream (its scratch may grow)") ? 1 : 0;
     const size_t rows = n, need[P_COUNT] = {rows * gq_t->O * 4,       rows * KH * hd * 4,     rows * KH * hd * 4,
                                             rows * h->H * hd * 4,     rows * h->H * hd * 4,
                                             coli_hip_attn_paged_work(p, &own)};

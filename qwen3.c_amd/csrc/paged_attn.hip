@@ -247,6 +247,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
     // the units of all rows in one line: a thread has `per` rows
     const int per = (a.n + kThreads - 1) / kThreads;
     long mine = 0, total = 0;
+#pragma unroll 4
     for (int i = 0; i < per; i++) {
         const int r = tid * per + i;
         int s = -1;
@@ -769,6 +770,7 @@ bool attn_paged(const PoolView &pv, const HeadsView &hv, int dtype, int layer, c
     while ((1L << a.shift) < pv.page) a.shift++;
     a.magic = (unsigned)(((1ULL << 32) * ((1ULL << a.shift) - pv.page)) / pv.page + 1);
     const long cap = (long)pv.max_pages * pv.page, len = max_len > 0 && max_len < cap ? max_len : cap;
+    if (((cap + keys - 1) / keys + 8) * a.khv >= 1L << 31) return paged_refuse("a sequence of too many units");
     const long units = ((len + keys - 1) / keys) * a.khv * (long)n;   // blocks beyond these would cut setups only
     const int blocks = (int)(units < most ? units : most);
     a.by_row = n * (long)a.khv <= blocks;

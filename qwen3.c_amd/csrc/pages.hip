@@ -16,7 +16,8 @@
 namespace coli {
 
 constexpr int kPgThreads = 1024;     // the bookkeeping block
-constexpr int kPgMaxN = 4096;        // sequences of one call (their offsets are held in LDS)
+constexpr int kTakeN = 4;            // sequences of a thread of pages_take
+constexpr int kPgMaxN = kTakeN * kPgThreads;   // of a call
 constexpr int kCopyThreads = 256;
 constexpr long kCopyPiece = 16384;   // bytes of a page that one block copies at a time
 
@@ -34,7 +35,7 @@ bool pool_view(const ColiHipPages *p, PoolView &v) {
     if (p->page < 1 || p->page > 4096) return paged_refuse("page size not in 1..4096");
     if (p->KH < 1 || p->KH > 1024 || p->n_layers < 1 || p->n_layers > 4096) return paged_refuse("heads or layers");
     if (p->n_pages < 1 || p->n_seqs < 1 || p->max_pages < 1) return paged_refuse("empty pool");
-    if ((long)p->max_pages * p->page >= 1L << 31 || p->n_pages > 1 << 30) return paged_refuse("pool too large");
+    if ((long)p->max_pages * p->page > 1L << 30 || p->n_pages > 1 << 30) return paged_refuse("pool too large");
     if ((uintptr_t)p->data % 16) return paged_refuse("pool data not aligned to 16 bytes");
     v.data = (char *)p->data;
     v.table = p->table, v.lens = p->lens, v.refs = p->refs, v.used = p->used, v.state = p->state, v.work = p->work;
@@ -101,114 +102,149 @@ enum { kTakeAppend = 0, kTakeShare = 1, kTakeCopy = 2 };
 // One block.  Append: sequence b[i] grows by count[i] positions (NULL: 1).  Fork: b[i] becomes
 // as long as a[i]; its new pages are the last, partly filled one (share) or all of them (copy).
 // Nothing changes unless the whole call can be done.
-__global__ __launch_bounds__(kPgThreads) void pages_take(PoolView p, const int *__restrict__ a,
-                                                         const int *__restrict__ b, const int *__restrict__ count,
-                                                         int n, int mode) {
-    constexpr int kHash = 2 * kPgMaxN;
-    __shared__ int s_off[kPgMaxN + 1];
-    __shared__ int s_list[kPgMaxN];   // the new pages, where they are few
-    __shared__ int s_hash[kHash];     // the sequences named so far
-    __shared__ int s_wave[kPgThreads / 64];
-    __shared__ int s_err;
-    const int tid = threadIdx.x, words = (p.n_pages + 31) / 32;
-    const unsigned word0 = tid < words ? used_word(p, tid) : ~0u;
-    if (tid == 0) s_err = 0;
-    for (int i = tid; i < kHash; i += kPgThreads) s_hash[i] = -1;
-    __syncthreads();
-    // what each needs
-    int err = 0;
-    for (int i = tid; i < n; i += kPgThreads) {
-        const int s = b[i], f = mode == kTakeAppend ? s : a[i];
-        int need = 0;
-        if (s < -1 || s >= p.n_seqs || f < -1 || f >= p.n_seqs) {
+// A chain of latencies (names, lengths, table) with three barriers: the scan that places the needs
+// also ranks the free pages of the first T words of the bitmap.  T = 512 where four words a
+// thread cover the pool, 1024 otherwise (60 forks in a pool of 13000 pages: 6.2 us with 512 threads, 7.7
+// with 1024; 20 sequences of 2200 pages in all: 11.0 both, 13.5 with 256).
+template <int T>
+__global__ __launch_bounds__(T) void pages_take(PoolView p, const int *__restrict__ a, const int *__restrict__ b,
+                                                const int *__restrict__ count, int n, int mode) {
+    constexpr int kMax = kTakeN * T, kHash = 2 * kMax, kW = T / 64;
+    __shared__ int s_off[kMax + 1];    // sequence i's new pages: [s_off[i], s_off[i + 1])
+    __shared__ int s_first[kMax];      // and its first new table entry
+    __shared__ int s_list[kMax];       // the new pages, where they are that few
+    __shared__ int s_hash[kHash];      // the sequences named so far
+    __shared__ long s_need[kW];
+    __shared__ int s_free[kW], s_more[kW], s_err[kW];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, words = (p.n_pages + 31) / 32;
+    const unsigned fr0 = tid < words ? ~used_word(p, tid) : 0u;
+    for (int i = tid; i < kHash; i += T) s_hash[i] = -1;
+    int more = 0;   // free pages past the first T words
+    for (int w = tid + T; w < words; w += T) more += __popc(~used_word(p, w));
+    const long most = (long)p.max_pages * p.page;
+    // what each needs: a thread has kTakeN neighbours
+    int s[kTakeN], need[kTakeN], grown[kTakeN], first[kTakeN], err = 0;
+#pragma unroll
+    for (int k = 0; k < kTakeN; k++) {
+        const int i = tid * kTakeN + k;
+        s[k] = -1, need[k] = grown[k] = first[k] = 0;
+        if (i >= n) continue;
+        const int to = b[i], from = mode == kTakeAppend ? to : a[i];
+        if (to < -1 || to >= p.n_seqs || from < -1 || from >= p.n_seqs) {
             err |= kPgIndex;
-        } else if (s >= 0 && f >= 0) {
-            unsigned at = (unsigned)s * 2654435761u % kHash;
-            for (;;) {   // ends: twice as many places as sequences
-                const int old = atomicCAS(&s_hash[at], -1, s);
-                if (old == s) err |= kPgTwice;
-                if (old == -1 || old == s) break;
-                at = (at + 1) % kHash;
-            }
-            const int len = p.lens[s];
-            const long most = (long)p.max_pages * p.page;
+        } else if (to >= 0 && from >= 0) {
+            s[k] = to;
+            const int len = p.lens[to];
             if (len < 0 || len > most) err |= kPgIndex;
             if (mode == kTakeAppend) {
                 const int c = count ? count[i] : 1;
-                if (c < 0)
+                if (c < 0) {
                     err |= kPgIndex;
-                else if ((long)len + c > most)
+                } else if ((long)len + c > most) {
                     err |= kPgRow;
-                else
-                    need = pages_of(len + c, p.page) - pages_of(len, p.page);
+                } else {
+                    grown[k] = len + c;
+                    first[k] = pages_of(len, p.page);
+                    need[k] = pages_of(len + c, p.page) - first[k];
+                }
             } else {
-                const int from = p.lens[f];
-                if (len != 0 || s == f) err |= kPgTwice;
-                if (from < 0 || from > most) err |= kPgIndex;
-                need = mode == kTakeCopy ? pages_of(from, p.page) : from % p.page != 0;
+                grown[k] = p.lens[from];
+                if (len != 0 || to == from) err |= kPgTwice;
+                if (grown[k] < 0 || grown[k] > most) err |= kPgIndex;
+                first[k] = mode == kTakeCopy ? 0 : grown[k] / p.page;
+                need[k] = pages_of(grown[k], p.page) - first[k];
             }
         }
-        s_off[i] = need;
     }
     __syncthreads();
-    // free pages, and the need: each thread sums four neighbours (both at most n_pages, or an error)
-    int nfree = 32 - __popc(word0), total_free, total = 0;
-    for (int w = tid + kPgThreads; w < words; w += kPgThreads) nfree += 32 - __popc(used_word(p, w));
-    block_scan(nfree, s_wave, &total_free);
-    int v[kPgMaxN / kPgThreads], mine = 0, full = 0;
+    long mine = 0;
 #pragma unroll
-    for (int k = 0; k < kPgMaxN / kPgThreads; k++) {
-        const int i = tid * (kPgMaxN / kPgThreads) + k;
-        v[k] = i < n ? s_off[i] : 0;
-        if (v[k] > total_free) full = 1, v[k] = 0;
-        mine += v[k];
-        if (mine > total_free) full = 1, mine = 0;   // keeps the sums below 2^31
+    for (int k = 0; k < kTakeN; k++) {
+        mine += need[k];
+        if (s[k] < 0) continue;
+        unsigned at = (unsigned)s[k] * 2654435761u % kHash;
+        for (;;) {   // ends: twice as many places as sequences
+            const int old = atomicCAS(&s_hash[at], -1, s[k]);
+            if (old == s[k]) err |= kPgTwice;
+            if (old == -1 || old == s[k]) break;
+            at = (at + 1) % kHash;
+        }
     }
-    // 1024 partial sums of at most 2^30 each: summed in 64 bits for the check
-    __shared__ unsigned long long s_total;
-    if (tid == 0) s_total = 0;
+    long x = mine;
+    int f = __popc(fr0);
+    const int f0 = f;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const long y = __shfl_up(x, o);
+        const int g = __shfl_up(f, o);
+        if (lane >= o) x += y, f += g;
+        more += __shfl_xor(more, o);
+        err |= __shfl_xor(err, o);
+    }
+    if (lane == 63) s_need[wave] = x, s_free[wave] = f, s_more[wave] = more, s_err[wave] = err;
     __syncthreads();
-    if (mine || full) atomicAdd(&s_total, (unsigned long long)mine + (full ? 1ull << 40 : 0));
-    if (err) atomicOr(&s_err, err);
-    __syncthreads();
-    if (tid == 0 && !s_err && s_total > (unsigned long long)total_free) s_err = kPgFull;
-    __syncthreads();
-    if (s_err) {
+    long total = 0, off = x - mine;
+    int found = 0, rank = f - f0, rest = 0;
+    err = 0;
+    for (int w = 0; w < kW; w++) {
+        off += w < wave ? s_need[w] : 0;
+        rank += w < wave ? s_free[w] : 0;
+        total += s_need[w], found += s_free[w], rest += s_more[w], err |= s_err[w];
+    }
+    if (!err && total > (long)found + rest) err = kPgFull;
+    if (err) {
         if (tid == 0) {
-            atomicOr(&p.state[kStErr], s_err);
+            atomicOr(&p.state[kStErr], err);
             p.state[kStGo] = 0;
         }
         return;
     }
-    int at = block_scan(mine, s_wave, &total);
+    // the lengths (all were read before the barrier: a fork's source may be another's target)
 #pragma unroll
-    for (int k = 0; k < kPgMaxN / kPgThreads; k++) {
-        const int i = tid * (kPgMaxN / kPgThreads) + k;
-        if (i < n) s_off[i] = at;
-        at += v[k];
+    for (int k = 0; k < kTakeN; k++) {
+        const int i = tid * kTakeN + k;
+        if (i < n) s_off[i] = (int)off, s_first[i] = first[k];
+        off += need[k];
+        if (s[k] >= 0) p.lens[s[k]] = grown[k];
     }
-    if (tid == 0) s_off[n] = total;
-    __syncthreads();
+    if (tid == 0) s_off[n] = (int)total, p.state[kStGo] = 1;
     // the lowest `total` free pages, in order, into the list
-    int *list = total <= kPgMaxN ? s_list : p.work;
-    for (int w0 = 0, base = 0; base < total && w0 < words; w0 += kPgThreads) {
+    int *list = total <= kMax ? s_list : p.work;
+    unsigned fr = fr0;
+    for (int w0 = 0, base = 0;;) {
         const int w = w0 + tid;
-        unsigned fr = !w0 ? ~word0 : w < words ? ~used_word(p, w) : 0u;
-        int found;
-        int r = base + block_scan(__popc(fr), s_wave, &found);
         unsigned taken = 0;
-        while (fr && r < total) {
+        while (fr && rank < total) {
             const int bit = __ffs(fr) - 1;
-            list[r++] = w * 32 + bit;
+            list[rank++] = w * 32 + bit;
             taken |= 1u << bit;
             fr &= fr - 1;
         }
         if (taken) p.used[w] |= taken;
         base += found;
+        w0 += T;
+        if (base >= total || w0 >= words) break;   // alike in every thread
+        fr = w0 + tid < words ? ~used_word(p, w0 + tid) : 0u;
+        f = __popc(fr);
+        rank = f;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int g = __shfl_up(rank, o);
+            if (lane >= o) rank += g;
+        }
+        __syncthreads();
+        if (lane == 63) s_free[wave] = rank;
+        __syncthreads();
+        rank += base - f;
+        found = 0;
+        for (int v = 0; v < kW; v++) {
+            rank += v < wave ? s_free[v] : 0;
+            found += s_free[v];
+        }
     }
     __syncthreads();
     // each page to its table entry
-    for (int r = tid; r < total; r += kPgThreads) {
+    for (int r = tid; r < (int)total; r += T) {
         int lo = 0, hi = n;   // the last i with s_off[i] <= r
         while (hi - lo > 1) {
             const int m = (lo + hi) / 2;
@@ -217,29 +253,10 @@ __global__ __launch_bounds__(kPgThreads) void pages_take(PoolView p, const int *
             else
                 hi = m;
         }
-        const int s = b[lo], k = r - s_off[lo], pg = list[r];
-        const int first = mode == kTakeAppend ? pages_of(p.lens[s], p.page)
-                        : mode == kTakeShare  ? p.lens[a[lo]] / p.page
-                                              : 0;
-        p.table[(size_t)s * p.max_pages + first + k] = pg;
+        const int pg = list[r];
+        p.table[(size_t)b[lo] * p.max_pages + s_first[lo] + r - s_off[lo]] = pg;
         p.refs[pg] = 1;
     }
-    // the lengths, all read before the first is written: a fork's source may be another's target
-    int len[kPgMaxN / kPgThreads];
-#pragma unroll
-    for (int k = 0; k < kPgMaxN / kPgThreads; k++) {
-        const int i = tid + k * kPgThreads;
-        len[k] = -1;
-        if (i >= n) continue;
-        const int s = b[i], f = mode == kTakeAppend ? s : a[i];
-        if (s < 0 || f < 0) continue;
-        len[k] = mode == kTakeAppend ? p.lens[s] + (count ? count[i] : 1) : p.lens[f];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kPgMaxN / kPgThreads; k++)
-        if (len[k] >= 0) p.lens[b[tid + k * kPgThreads]] = len[k];
-    if (tid == 0) p.state[kStGo] = 1;
 }
 
 // ---------------------------------------------------------------- copying
@@ -440,12 +457,19 @@ static bool take_args(const ColiHipPages *p, PoolView &v, const void *seq, int n
     return !n || seq || paged_refuse("NULL sequence list");
 }
 
+static void take(const PoolView &v, const int *a, const int *b, const int *count, int n, int mode, hipStream_t st) {
+    if (n <= kTakeN * 512 && v.n_pages <= 512 * 32 * 4)
+        hipLaunchKernelGGL(pages_take<512>, dim3(1), dim3(512), 0, st, v, a, b, count, n, mode);
+    else
+        hipLaunchKernelGGL(pages_take<kPgThreads>, dim3(1), dim3(kPgThreads), 0, st, v, a, b, count, n, mode);
+}
+
 COLI_API int coli_hip_pages_append(const ColiHipPages *p, const int *d_seq, const int *d_count, int n, void *stream_) {
     PoolView v;
     hipStream_t st;
     if (!take_args(p, v, d_seq, n) || !paged_stream(stream_, st)) return 0;
     if (!n) return 1;
-    hipLaunchKernelGGL(pages_take, dim3(1), dim3(kPgThreads), 0, st, v, d_seq, d_seq, d_count, n, (int)kTakeAppend);
+    take(v, d_seq, d_seq, d_count, n, kTakeAppend, st);
     return paged_launched("pages append") ? 1 : 0;
 }
 
@@ -455,12 +479,10 @@ COLI_API int coli_hip_pages_fork(const ColiHipPages *p, const int *d_src, const 
     hipStream_t st;
     if (!take_args(p, v, d_src && d_dst ? d_src : nullptr, n) || !paged_stream(stream_, st)) return 0;
     if (!n) return 1;
-    hipLaunchKernelGGL(pages_take, dim3(1), dim3(kPgThreads), 0, st, v, d_src, d_dst, (const int *)nullptr, n,
-                       share ? (int)kTakeShare : (int)kTakeCopy);
+    take(v, d_src, d_dst, nullptr, n, share ? kTakeShare : kTakeCopy, st);
     const int pieces = pieces_of(v);
     // share: a page's pieces; copy: enough blocks for the whole card
-    long y = share ? pieces : (8L * n_cu() + n - 1) / n;
-    y = y < 1 ? 1 : y > 2048 ? 2048 : y;
+    const long most = (65536 + n - 1) / n, want = share ? pieces : (8L * n_cu() + n - 1) / n, y = want < most ? want : most;
     hipLaunchKernelGGL(pages_fork_copy, dim3(n, (unsigned)y), dim3(kCopyThreads), 0, st, v, d_src, d_dst, share ? 1 : 0,
                        pieces);
     return paged_launched("pages fork") ? 1 : 0;

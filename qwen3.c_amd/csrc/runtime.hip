@@ -89,7 +89,7 @@ bool scratch(void **p, size_t *cap, size_t need) {
     if (need <= *cap && *p) return true;
     size_t want = need < 4096 ? 4096 : need;
     if (*p) {
-        hipError_t e = hipStreamSynchronize(G.st);   // old buffer may still be in use
+        hipError_t e = hipDeviceSynchronize();   // old buffer may still be in use, on any stream
         if (e != hipSuccess) return fail("scratch sync", e);
         (void)hipFree(*p);
         *p = nullptr;
@@ -98,6 +98,7 @@ bool scratch(void **p, size_t *cap, size_t need) {
     hipError_t e = hipMalloc(p, want);
     if (e != hipSuccess) return fail("scratch hipMalloc", e);
     e = hipMemsetAsync(*p, 0, want, G.st);
+    if (e == hipSuccess) e = hipStreamSynchronize(G.st);   // the first use may be on a caller's stream
     if (e != hipSuccess) return fail("scratch memset", e);
     *cap = want;
     return true;

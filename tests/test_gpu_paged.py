@@ -440,6 +440,30 @@ def test_attn_long(mod, lib, dev, dtype, H, KH, hd, n, length):
     assert torch.equal(again, first)   # the same call twice: the same bits
 
 
+@pytest.mark.parametrize("dtype,KH,hd,n", [(BF16, 2, 64, 700), (F32, 1, 128, 300), (F16, 2, 256, 257), (BF16, 1, 8, 5000)],
+                         ids=lambda v: str(v))
+def test_attn_many_rows(mod, lib, dev, dtype, KH, hd, n):
+    """More rows than a block has threads: drafts and short chats, rows of no sequence at both
+    ends and between, several rows a sequence."""
+    rng = np.random.default_rng(n)
+    lens = [int(x) for x in rng.integers(0, 150, 40)]
+    lens[7] = 2000
+    pool = Pool(mod, lib, dev, dtype, 1, KH, hd, 16, sum(-(-x // 16) for x in lens) + 1, 40, 130, seed=3)
+    pool.place(lens)
+    a = Attn(mod, lib, dev, pool, 4 * KH, False, seed=1)
+    seq = [int(x) for x in rng.integers(-1, 40, n)]
+    seq[:3], seq[-2:] = [-1, -1, 7], [7, -1]
+    pos = [int(rng.integers(-1, lens[s])) if s >= 0 else 5 for s in seq]
+    q, raw = a.rows(n)
+    got = a.run(q, raw, seq, pos)
+    assert lib.pages_status(pool.c)[1] == 0
+    check = sorted(set(range(0, n, max(1, n // 250))) | {0, 1, 2, n - 2, n - 1})
+    pool.data = pool.data.cpu()
+    a.check(got[check], q[check], raw[check], [seq[i] for i in check], [pos[i] + 1 for i in check])
+    rest = [i for i in range(n) if seq[i] < 0 or pos[i] < 0]
+    assert bool((got[rest] == torch.tensor([77.0 if seq[i] < 0 else 0.0 for i in rest])[:, None, None]).all())
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "f16", "f32"])
 def test_attn_extremes(mod, lib, dev, dtype):
     """Scores far apart, all alike, queries of 0, large and tiny; tiny and large values; keys in
@@ -536,7 +560,8 @@ def test_attn_refusals(mod, lib, dev):
     w, nb = addr(a.work), a.work.numel()
     ok = (P, h, 0, addr(q), None, addr(s), None, 1, 0, addr(out), w, nb, None)
     assert L.coli_hip_attn_paged(*ok) == 1
-    for i, v in ((1, None), (2, 1), (2, -1), (3, None), (5, None), (7, -1), (9, None), (10, None), (10, w + 8),
+    for i, v in ((1, None), (2, 1), (2, -1), (3, None), (5, None), (7, -1), (7, (1 << 20) + 1), (9, None),
+                 (9, addr(out) + 4), (10, None), (10, w + 8),
                  (11, nb - 1)):
         args = list(ok)
         args[i] = v
@@ -737,7 +762,20 @@ def test_gqa_paged_matches_dense(mod, lib, gen, dev):
         Kd, Vd = lib.kv_read(layer, h * max_t, S, hd, hd)
         Kp, Vp = pool.rows(0, 1, S, 0)[h].numpy(), pool.rows(0, 1, S, 1)[h].numpy()
         assert np.max(np.abs(Kd - Kp)) <= 1e-4 * np.max(np.abs(Kd)) and np.max(np.abs(Vd - Vp)) <= 1e-5 * np.max(np.abs(Vd))
+    side = torch.cuda.Stream()   # on a caller's stream, padded: the same rows
+    again, more = torch.full((S, D), 3.0, device=dev), ints([1] * (S - 1) + [-1], dev)
+    torch.cuda.synchronize()
+    lib.gqa_paged_dev(pool.c, heads, 0, addr(x), tq, tk, tv, to, addr(more), addr(pos), S, 0, addr(again),
+                      side.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(again[:S - 1], out[:S - 1]) and not bool(again[S - 1].any())
     L, P, h = lib.L, C.byref(pool.c), C.byref(heads)
+    graph = torch.cuda.CUDAGraph()   # refused while captured, with nothing broken
+    with torch.cuda.graph(graph, stream=side):
+        again.zero_()
+        assert L.coli_hip_gqa_paged(P, h, 0, addr(x), D, tq.handle, tk.handle, tv.handle, to.handle, addr(seq),
+                                    addr(pos), S, S, addr(out), torch.cuda.current_stream().cuda_stream) == 0
+    assert lib.available()
     ok = [P, h, 0, addr(x), D, tq.handle, tk.handle, tv.handle, to.handle, addr(seq), addr(pos), S, S, addr(out), None]
     for i, v in ((0, None), (1, None), (2, 1), (3, None), (4, D + 1), (5, tk.handle), (6, None), (7, tq.handle),
                  (9, None), (11, -1), (13, None)):
