@@ -235,8 +235,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
     constexpr int kQWords = kNT * 16 * kQRow, kOffWords = 2 * (kWindow + kPad), kSum = HD * 16;
     // q and the offsets of the keys' rows, then the waves' sums
     __shared__ __attribute__((aligned(16))) unsigned s_mem[kQWords + kOffWords > 2 * kSum ? kQWords + kOffWords : 2 * kSum];
-    __shared__ int s_cnt[kThreads], s_seq[kThreads], s_row;
-    __shared__ long s_wave[kWaves], s_first;
+    __shared__ int s_cnt[kThreads], s_seq[kThreads], s_wave[kWaves], s_row, s_first;
     __shared__ float s_inv[kGroup], s_m[kWaves][kGroup], s_l[kWaves][kGroup];
     unsigned *const s_q = s_mem;
     long *const s_off = (long *)(s_mem + kQWords);
@@ -246,7 +245,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
 
     // the units of all rows in one line: a thread has `per` rows
     const int per = (a.n + kThreads - 1) / kThreads;
-    long mine = 0, total = 0;
+    int mine = 0, total = 0;
 #pragma unroll 4
     for (int i = 0; i < per; i++) {
         const int r = tid * per + i;
@@ -256,25 +255,25 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         s_seq[tid] = s;
         if (a.by_row && !blockIdx.x && r < a.n && cnt < 0)   // no block has this row
             for (int k = 0; k < a.khv; k++) a.cut[r * a.khv + k].parts = 0;
-        mine += (long)units_of<kKeys, kSetup>(cnt) * a.khv;
+        mine += units_of<kKeys, kSetup>(cnt) * a.khv;
     }
-    long x = mine;
+    int x = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const long y = __shfl_up(x, o);
+        const int y = __shfl_up(x, o);
         if (lane >= o) x += y;
     }
     if (lane == 63) s_wave[wave] = x;
     __syncthreads();
-    long before = x - mine;
+    int before = x - mine;
+#pragma unroll
     for (int w = 0; w < kWaves; w++) {
         before += w < wave ? s_wave[w] : 0;
         total += s_wave[w];
     }
     total = uniform(total);
-    // (total + blocks - 1) / blocks: below 2^53 and a fraction of at least 1 / blocks from a whole number
-    const long share = uniform((long)((double)(total + gridDim.x - 1) / (double)gridDim.x));
-    const long u0 = blockIdx.x * share, end = min(total, u0 + share);
+    const int share = uniform((int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
+    const int u0 = min(total, (int)blockIdx.x * share), end = min(total, u0 + share);
     if (u0 >= end) {
         if (tid == 0 && !a.by_row) a.cut[blockIdx.x].parts = 0;
         return;
@@ -283,7 +282,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         int r = tid * per;
         for (int i = 1; i < per; i++) {
             int s;
-            const long k = (long)units_of<kKeys, kSetup>(row_count(p, a, r, s)) * a.khv;
+            const int k = units_of<kKeys, kSetup>(row_count(p, a, r, s)) * a.khv;
             if (before + k > u0) break;
             before += k;
             r++;
@@ -293,11 +292,11 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
     }
     __syncthreads();
     int r = uniform(s_row);
-    long first = uniform(s_first);   // units before row r
+    int first = uniform(s_first);   // units before row r
     Cut cut = {};
     int done = 0;   // whether the block has had a part before
 
-    for (long u = u0; u < end && r < a.n;) {
+    for (int u = u0; u < end && r < a.n;) {
         int s, cnt;
         if (per == 1) {
             s = s_seq[r];
@@ -308,14 +307,14 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         s = uniform(s);
         cnt = uniform(cnt);
         const int nc = chunks_of<kKeys>(cnt), nu = units_of<kKeys, kSetup>(cnt);
-        const long xx = u - first;
-        if (xx >= (long)nu * a.khv) {   // this row is done (or has none)
-            first += (long)nu * a.khv;
+        const int xx = u - first;
+        if (xx >= nu * a.khv) {   // this row is done (or has none)
+            first += nu * a.khv;
             r++;
             continue;
         }
-        const int hv = uniform((int)((unsigned)xx / (unsigned)nu)), x0 = (int)xx - hv * nu;
-        const int x1 = (int)min((long)nu, x0 + (end - u)), c0 = max(x0 - kSetup, 0), c1 = x1 - kSetup;
+        const int hv = uniform((int)((unsigned)xx / (unsigned)nu)), x0 = xx - hv * nu;
+        const int x1 = min(nu, x0 + (end - u)), c0 = max(x0 - kSetup, 0), c1 = x1 - kSetup;
         u += x1 - x0;
         if (c1 <= c0) continue;   // the keys are the next block's
         const int kh = uniform(hv / a.groups), h0 = (hv - kh * a.groups) * kGroup, hn = min(kGroup, G - h0);
@@ -583,18 +582,9 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
             s_m[wave][c] = m;
             s_l[wave][c] = l;
         }
-        float z = l;
-        if (!kWide) {
-#pragma unroll
-            for (int t = 0; t < kVS; t++)
-#pragma unroll
-                for (int e = 0; e < kVE; e++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) z = fmaf(acc[t][e][i], 0.f, z);
-        }
-        if (__syncthreads_or(!kWide && !(fabsf(z) < INFINITY))) {
-            slow_part<T>(p, h, a, r, s, kh, head, hn, cnt, from, last, whole, slot, s_o, &s_m[0][0]);
-        } else {
+        __syncthreads();
+        float z = 0.f;   // NaN when a result of this thread's is not finite
+        {
             const float M = fmaxf(fmaxf(s_m[0][c], s_m[1][c]), fmaxf(s_m[2][c], s_m[3][c]));
             const float f = m == M ? 1.f : __builtin_amdgcn_exp2f(m - M);
 #pragma unroll
@@ -635,6 +625,8 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
 #pragma unroll
                     for (int e = 0; e < kVE; e++) o[e] += at[256 * e] + at[kSum + 256 * e];
                 }
+#pragma unroll
+                for (int e = 0; e < kVE; e++) z = fmaf(o[e] + L, 0.f, z);
                 float *dst = a.part + (slot * kGroup + hh) * p.hd + d0;
                 if (whole) {
                     dst = a.out + ((long)r * h.H + head + hh) * p.hd + d0;
@@ -647,12 +639,14 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
 #pragma unroll
                 for (int e = 0; e < kVE; e += 4) *(float4 *)(dst + e) = *(const float4 *)(o + e);
             }
-            __syncthreads();   // the sums' place is the next part's q
         }
+        // the sums' place is the next part's q; 16-bit products that met an infinity or NaN: again
+        if (__syncthreads_or(!kWide && z != 0.f))
+            slow_part<T>(p, h, a, r, s, kh, head, hn, cnt, from, last, whole, slot, s_o, &s_m[0][0]);
         if (c0 == 0) {   // u is behind its unit c1
             cut = Cut{};
             if (c1 < nc) {
-                const int parts = (int)((double)(u + (nc - c1) - 1) / (double)share) - (int)blockIdx.x + 1;
+                const int parts = (int)((unsigned)(u + (nc - c1) - 1) / (unsigned)share) - (int)blockIdx.x + 1;
                 cut = Cut{r, (int)head, hn, parts, (int)blockIdx.x, (int)slot};
             }
             if (a.by_row && tid == 0) a.cut[r * a.khv + hv] = cut;
@@ -770,20 +764,32 @@ bool attn_paged(const PoolView &pv, const HeadsView &hv, int dtype, int layer, c
     while ((1L << a.shift) < pv.page) a.shift++;
     a.magic = (unsigned)(((1ULL << 32) * ((1ULL << a.shift) - pv.page)) / pv.page + 1);
     const long cap = (long)pv.max_pages * pv.page, len = max_len > 0 && max_len < cap ? max_len : cap;
-    if (((cap + keys - 1) / keys + 8) * a.khv >= 1L << 31) return paged_refuse("a sequence of too many units");
-    const long units = ((len + keys - 1) / keys) * a.khv * (long)n;   // blocks beyond these would cut setups only
-    const int blocks = (int)(units < most ? units : most);
-    a.by_row = n * (long)a.khv <= blocks;
-    switch (dtype) {
-    case COLI_HIP_F32: launch<COLI_HIP_F32, 16>(pv, hv, a, blocks, st); break;
-    case COLI_HIP_F16: launch_heads<COLI_HIP_F16>(pv, hv, a, blocks, st); break;
-    default: launch_heads<COLI_HIP_BF16>(pv, hv, a, blocks, st);
-    }
-    if (blocks > 1) {
-        // few cuts: blocks of 64 columns (16 parts at a time); else of a whole head
-        const int cuts = a.by_row ? n * a.khv : blocks, heads = G < kGroup ? G : kGroup;
-        const int cols = cuts * heads <= 512 ? 64 : pv.hd <= 64 ? 64 : pv.hd <= 128 ? 128 : 256;
-        hipLaunchKernelGGL(attn_join, dim3(cuts, heads, (pv.hd + cols - 1) / cols), dim3(kThreads), 0, st, pv, hv, a, cols);
+    // the units of a launch's rows are counted in 31 bits: more rows go in several launches
+    const long row = ((cap + keys - 1) / keys + 4) * a.khv;
+    if (row >= 1L << 30) return paged_refuse("a sequence of more than 2^30 units");
+    const int rows = (int)min((long)n, (1L << 30) / row);
+    for (int r = 0; r < n; r += rows) {
+        a.n = min(rows, n - r);
+        const long units = ((len + keys - 1) / keys) * a.khv * (long)a.n;   // more blocks would cut setups only
+        const int blocks = (int)(units < most ? units : most);
+        a.by_row = a.n * (long)a.khv <= blocks;
+        switch (dtype) {
+        case COLI_HIP_F32: launch<COLI_HIP_F32, 16>(pv, hv, a, blocks, st); break;
+        case COLI_HIP_F16: launch_heads<COLI_HIP_F16>(pv, hv, a, blocks, st); break;
+        default: launch_heads<COLI_HIP_BF16>(pv, hv, a, blocks, st);
+        }
+        if (blocks > 1) {
+            // few cuts: blocks of 64 columns (16 parts at a time); else of a whole head
+            const int cuts = a.by_row ? a.n * a.khv : blocks, heads = G < kGroup ? G : kGroup;
+            const int cols = cuts * heads <= 512 ? 64 : pv.hd <= 64 ? 64 : pv.hd <= 128 ? 128 : 256;
+            hipLaunchKernelGGL(attn_join, dim3(cuts, heads, (pv.hd + cols - 1) / cols), dim3(kThreads), 0, st, pv, hv, a,
+                               cols);
+        }
+        a.q += (size_t)a.n * hv.H * pv.hd;
+        a.out += (size_t)a.n * hv.H * pv.hd;
+        a.seq += a.n;
+        if (a.pos) a.pos += a.n;
+        if (a.gate) a.gate += a.n * hv.q_row;
     }
     return paged_launched("paged attention launch");
 }

@@ -464,6 +464,19 @@ def test_attn_many_rows(mod, lib, dev, dtype, KH, hd, n):
     assert bool((got[rest] == torch.tensor([77.0 if seq[i] < 0 else 0.0 for i in rest])[:, None, None]).all())
 
 
+def test_attn_rows_in_several_launches(mod, lib, dev):
+    """Table rows of 2^30 positions: four rows' units fill a launch's counter, ten rows take three
+    launches over one workspace."""
+    pool = Pool(mod, lib, dev, F32, 1, 16, 8, 4096, 12, 10, 1 << 18, seed=3)
+    lens = [4097, 1, 300, 0, 4096, 64, 65, 5000, 129, 4000]
+    pool.place(lens)
+    a = Attn(mod, lib, dev, pool, 16, True, seed=1)
+    q, raw = a.rows(10)
+    got = a.run(q, raw, list(range(10)))
+    a.check(got, q, raw, list(range(10)), lens)
+    assert lib.pages_status(pool.c)[1] == 0
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "f16", "f32"])
 def test_attn_extremes(mod, lib, dev, dtype):
     """Scores far apart, all alike, queries of 0, large and tiny; tiny and large values; keys in
