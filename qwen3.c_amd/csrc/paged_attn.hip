@@ -24,10 +24,17 @@
 // formula gives.
 //
 // Work: a unit is kKeys keys (a tile per wave) of a kv head, 64 KB or so; a (row, kv head) counts
-// kSetup units more, about what its q, row offsets and sums cost beside the keys (200 ragged rows
-// of 45 to 2900 keys: SETUPTIMES).  The units of all rows in one line are cut into equal shares, one
-// per block, whatever the lengths are.  A (row, kv head) that a border cuts goes through the
-// workspace, and attn_join joins its parts.
+// kSetup units more, about what its q, row offsets and sums cost beside the keys (200 ragged rows of
+// 45 to 2900 keys, 8 kv heads: 156 us without, 125 with one).  The units of all rows in one line
+// are cut into equal shares, one per block, whatever the lengths are.  A (row, kv head) that a
+// border cuts goes through the workspace, and attn_join joins its parts.
+//
+// Bound by the bytes of K and V where there are many: two rows of 120000 keys (2 kv heads of 256,
+// f16) 98 us, 5.0 TB/s (a large copy here moves 4.9); 48 rows of up to 16000 keys 70 us, 4.3; the 200
+// rows above 125 us, 4.6.  Bound by a chain of latencies where there are few: one row of 600 keys
+// 15 us, of which 4 are the join.  Tried and left out: 32-key tiles for heads of 256 (spills: 48 rows
+// 121 us against 78), more blocks per CU for heads of 128 (154 us with two, 165 with three), a join
+// by the last block to arrive (its fences and atomics take as long as the second launch).
 #include "paged.h"
 
 #include <math.h>
@@ -155,8 +162,8 @@ __device__ __forceinline__ float sum_pieces(float x) {
 }
 
 __device__ __forceinline__ float finish(float o, float l, int cnt, const float *gate, long at) {
-    const float d = gate ? l * (1.f + expf(-gate[at])) : l;
-    return cnt ? o / d : 0.f;
+    o = cnt ? o / l : 0.f;
+    return gate && cnt ? o / (1.f + expf(-gate[at])) : o;
 }
 
 // A part in plain fp32: keys [from, last) of the row, a key per wave at a time, four columns a

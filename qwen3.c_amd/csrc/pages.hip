@@ -8,6 +8,10 @@
 // call, counts are integers, and a page's bit falls with the count that reaches 0.  A page that
 // is not full belongs to one sequence alone (fork copies it), so a new position never lands in
 // a shared page.
+//
+// The copies are bound by their bytes: 20 of 40 sequences replaced with the pool closed up, 530 MB
+// moved, 227 us for the four launches (the move 197 us, 5.4 TB/s); six sequences copied whole, 209 MB,
+// 103 us (the copy 89).  60 forks that share their full pages: 16 us, three launches of 3 to 7 us.
 #include "paged.h"
 
 #include <stdio.h>

@@ -63,9 +63,8 @@ class Pool:
 
     def rows(self, layer, s, n, kv):
         """K (kv 0) or V rows 0..n-1 of sequence s in 64 bits [KH, n, hd], from the arrays."""
-        data, table = self.data.cpu(), self.table.cpu()
-        pg = table[s, :-(-n // self.page)].long()
-        x = data[pg, layer, kv]                      # [P, KH, page, hd]
+        pg = self.table[s, :-(-n // self.page)].long().to(self.data.device)
+        x = self.data[pg, layer, kv].cpu()           # [P, KH, page, hd]
         return x.permute(1, 0, 2, 3).reshape(self.KH, -1, self.hd)[:, :n].double()
 
 

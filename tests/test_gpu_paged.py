@@ -464,6 +464,47 @@ def test_attn_many_rows(mod, lib, dev, dtype, KH, hd, n):
     assert bool((got[rest] == torch.tensor([77.0 if seq[i] < 0 else 0.0 for i in rest])[:, None, None]).all())
 
 
+def test_offsets_past_32_bits(mod, lib, dev):
+    """A pool of 6.5 GB whose sequence lies at its far end: rows written, attended, copied there and
+    moved down from there."""
+    H, KH, hd, page, layers, n_pages = 8, 2, 256, 16, 10, 20_000
+    pool = Pool(mod, lib, dev, BF16, layers, KH, hd, page, n_pages, 3, 8, fill=False)
+    far = [n_pages - 1, n_pages - 7, n_pages - 3]
+    pool.table[0, :3] = ints(far, dev)
+    refs = np.zeros(n_pages, np.int32)
+    refs[far] = 1
+    refs[5] = 1   # page 5 is another's: the copies go around it
+    pool.table[2, 0], pool.lens[2] = 5, 3
+    pool.refs.copy_(torch.from_numpy(refs))
+    pool.used.copy_(torch.from_numpy(_paged.bitmap(refs)))
+    n = 40
+    pool.lens[0] = n
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(n, h * hd, generator=g) for h in (H, KH, KH))
+    d = [t.to(dev) for t in (q, k, v)]
+    heads = mod.Lib.heads(H=H, rot=0, interleaved=0, q_row=H * hd, q_head=hd, kv_row=KH * hd, eps=1e-6, rope_mag=1.0,
+                          scale=1.0 / 16)
+    out, s, p = torch.zeros(n, H, hd, device=dev), ints([0] * n, dev), ints(range(n), dev)
+    torch.cuda.synchronize()
+    lib.qk_rope_paged_dev(pool.c, heads, layers - 1, *(addr(t) for t in d), addr(s), addr(p), n, addr(out))
+    sync(lib)
+    K, V = (pool.rows(layers - 1, 0, n, i) for i in (0, 1))
+    assert torch.equal(K, k.view(n, KH, hd).bfloat16().double().transpose(0, 1))
+    assert torch.equal(V, v.view(n, KH, hd).bfloat16().double().transpose(0, 1))
+    a = Attn(mod, lib, dev, pool, H, False)
+    qq, raw = a.rows(2)
+    a.check(a.run(qq, raw, [0, 0], [n - 1, 17], layer=layers - 1), qq, raw, [0, 0], [n, 18], layer=layers - 1)
+    lib.pages_fork(pool.c, addr(x := ints([0], dev)), addr(y := ints([1], dev)), 1, False)
+    lib.sync()
+    assert pool.table[1, :4].tolist() == [0, 1, 2, -1]
+    assert torch.equal(pool.rows(layers - 1, 1, n, 0), K) and torch.equal(pool.rows(layers - 1, 1, n, 1), V)
+    lib.pages_compact(pool.c)
+    lib.sync()   # 7 pages: those past them, in order, into 3, 4 and 6; page 5 stays
+    assert pool.table[0, :4].tolist() == [6, 3, 4, -1] and pool.table[2, 0] == 5
+    assert torch.equal(pool.rows(layers - 1, 0, n, 0), K) and torch.equal(pool.rows(layers - 1, 0, n, 1), V)
+    assert lib.pages_status(pool.c) == (n_pages - 7, 0)
+
+
 def test_attn_rows_in_several_launches(mod, lib, dev):
     """Table rows of 2^30 positions: four rows' units fill a launch's counter, ten rows take three
     launches over one workspace."""
