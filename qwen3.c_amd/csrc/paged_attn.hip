@@ -241,7 +241,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
     constexpr int kQRow = kWide ? HD + 4 : HD / 2 + 4;                             // words of a q row in LDS
     constexpr int kQWords = kNT * 16 * kQRow, kOffWords = 2 * (kWindow + kPad), kSum = HD * 16;
     // q and the offsets of the keys' rows, then the waves' sums
-    __shared__ __attribute__((aligned(16))) unsigned s_mem[kQWords + kOffWords > 2 * kSum ? kQWords + kOffWords : 2 * kSum];
+    __shared__ __attribute__((aligned(16))) unsigned s_mem[kQWords + kOffWords > kWaves * kSum ? kQWords + kOffWords : kWaves * kSum];
     __shared__ int s_cnt[kThreads], s_seq[kThreads], s_wave[kWaves], s_row, s_first;
     __shared__ float s_inv[kGroup], s_m[kWaves][kGroup], s_l[kWaves][kGroup];
     unsigned *const s_q = s_mem;
@@ -250,19 +250,19 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 15, g = lane >> 4;
     const int G = h.H / p.KH;
 
-    // the units of all rows in one line: a thread has `per` rows
-    const int per = (a.n + kThreads - 1) / kThreads;
-    int mine = 0, total = 0;
+    // The units of all rows in one line: a thread has `per` rows; 64 rows or fewer every wave lines
+    // up for itself, a lane a row.
+    const bool few = a.n <= 64;
+    const int per = few ? 1 : (a.n + kThreads - 1) / kThreads, t0 = few ? lane : tid * per;
+    int mine = 0, total = 0, cnt_t = -1, seq_t = -1;
 #pragma unroll 4
     for (int i = 0; i < per; i++) {
-        const int r = tid * per + i;
-        int s = -1;
-        const int cnt = r < a.n ? row_count(p, a, r, s) : -1;
-        s_cnt[tid] = cnt;
-        s_seq[tid] = s;
-        if (a.by_row && !blockIdx.x && r < a.n && cnt < 0)   // no block has this row
+        const int r = t0 + i;
+        seq_t = -1;
+        cnt_t = r < a.n ? row_count(p, a, r, seq_t) : -1;
+        if (a.by_row && !blockIdx.x && r < a.n && cnt_t < 0)   // no block has this row
             for (int k = 0; k < a.khv; k++) a.cut[r * a.khv + k].parts = 0;
-        mine += units_of<kKeys, kSetup>(cnt) * a.khv;
+        mine += units_of<kKeys, kSetup>(cnt_t) * a.khv;
     }
     int x = mine;
 #pragma unroll
@@ -270,49 +270,65 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         const int y = __shfl_up(x, o);
         if (lane >= o) x += y;
     }
-    if (lane == 63) s_wave[wave] = x;
-    __syncthreads();
     int before = x - mine;
+    if (few) {
+        total = __builtin_amdgcn_readlane(x, 63);
+    } else {
+        s_cnt[tid] = cnt_t;
+        s_seq[tid] = seq_t;
+        if (lane == 63) s_wave[wave] = x;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) {
-        before += w < wave ? s_wave[w] : 0;
-        total += s_wave[w];
+        for (int w = 0; w < kWaves; w++) {
+            before += w < wave ? s_wave[w] : 0;
+            total += s_wave[w];
+        }
+        total = uniform(total);
     }
-    total = uniform(total);
     const int share = uniform((int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
     const int u0 = min(total, (int)blockIdx.x * share), end = min(total, u0 + share);
     if (u0 >= end) {
         if (tid == 0 && !a.by_row) a.cut[blockIdx.x].parts = 0;
         return;
     }
-    if (before <= u0 && u0 < before + mine) {   // unit u0 is in a row of this thread's
-        int r = tid * per;
-        for (int i = 1; i < per; i++) {
-            int s;
-            const int k = units_of<kKeys, kSetup>(row_count(p, a, r, s)) * a.khv;
-            if (before + k > u0) break;
-            before += k;
-            r++;
+    // the row of unit u0, and the units before it
+    int r, first;
+    const bool mine0 = before <= u0 && u0 < before + mine;
+    if (few) {
+        r = __ffsll((unsigned long long)__ballot(mine0)) - 1;
+        first = __builtin_amdgcn_readlane(before, r);
+    } else {
+        if (mine0) {
+            int k = tid * per;
+            for (int i = 1; i < per; i++) {
+                int s;
+                const int units = units_of<kKeys, kSetup>(row_count(p, a, k, s)) * a.khv;
+                if (before + units > u0) break;
+                before += units;
+                k++;
+            }
+            s_row = k;
+            s_first = before;
         }
-        s_row = r;
-        s_first = before;
+        __syncthreads();
+        r = uniform(s_row);
+        first = uniform(s_first);
     }
-    __syncthreads();
-    int r = uniform(s_row);
-    int first = uniform(s_first);   // units before row r
     Cut cut = {};
     int done = 0;   // whether the block has had a part before
 
     for (int u = u0; u < end && r < a.n;) {
         int s, cnt;
-        if (per == 1) {
-            s = s_seq[r];
-            cnt = s_cnt[r];
+        if (few) {
+            s = __builtin_amdgcn_readlane(seq_t, r);
+            cnt = __builtin_amdgcn_readlane(cnt_t, r);
+        } else if (per == 1) {
+            s = uniform(s_seq[r]);
+            cnt = uniform(s_cnt[r]);
         } else {
-            cnt = row_count(p, a, r, s);
+            cnt = uniform(row_count(p, a, r, s));
+            s = uniform(s);
         }
-        s = uniform(s);
-        cnt = uniform(cnt);
         const int nc = chunks_of<kKeys>(cnt), nu = units_of<kKeys, kSetup>(cnt);
         const int xx = u - first;
         if (xx >= nu * a.khv) {   // this row is done (or has none)
@@ -582,7 +598,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
 
         const bool whole = c0 == 0 && c1 == nc;
         const long slot = 2L * blockIdx.x + done;
-        // the four waves' parts under one maximum
+        // the four waves' parts
         l += other16(l);
         l += other32(l);
         if (g == 0) {
@@ -592,37 +608,22 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         __syncthreads();
         float z = 0.f;   // NaN when a result of this thread's is not finite
         {
-            const float M = fmaxf(fmaxf(s_m[0][c], s_m[1][c]), fmaxf(s_m[2][c], s_m[3][c]));
-            const float f = m == M ? 1.f : __builtin_amdgcn_exp2f(m - M);
+            float *so = s_o + wave * kSum + 4 * lane;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float fr = __shfl(f, 4 * g + i);   // of row 4 g + i
-#pragma unroll
-                for (int t = 0; t < kVS; t++)
-#pragma unroll
-                    for (int e = 0; e < kVE; e++) acc[t][e][i] *= fr;
-            }
-            // waves 2 and 3 into 0 and 1, whose sums the threads then add and write
-            float *so = s_o + (wave & 1) * kSum + 4 * lane;
-            if (wave >= 2) {
-#pragma unroll
-                for (int t = 0; t < kVS * kVE; t++) *(v4f *)(so + 256 * t) = acc[t / kVE][t % kVE];
-            }
-            __syncthreads();
-            if (wave < 2) {
-#pragma unroll
-                for (int t = 0; t < kVS * kVE; t++) *(v4f *)(so + 256 * t) = acc[t / kVE][t % kVE] + *(v4f *)(so + 256 * t);
-            }
+            for (int t = 0; t < kVS * kVE; t++) *(v4f *)(so + 256 * t) = acc[t / kVE][t % kVE];
             __syncthreads();
             // a thread: head hh's kVE columns from d0.  Rows of one head's pieces are GS apart.
-            for (int i = tid; i < hn * kVS * 16; i += kThreads) {
-                const int hh = i / 16 % hn, t = i / 16 / hn, d0 = (16 * t + (i & 15)) * kVE;
-                if (!kExact && d0 >= p.hd) continue;
-                float mw[kWaves], M = -INFINITY, L = 0.f, o[kVE];
+            for (int i = tid; i < GS * kVS * 16; i += kThreads) {
+                const int hh = i / 16 % GS, t = i / 16 / GS, d0 = (16 * t + (i & 15)) * kVE;
+                if (hh >= hn || (!kExact && d0 >= p.hd)) continue;
+                float f[kWaves], M = -INFINITY, L = 0.f, o[kVE];
 #pragma unroll
-                for (int w = 0; w < kWaves; w++) M = fmaxf(M, mw[w] = s_m[w][hh]);
+                for (int w = 0; w < kWaves; w++) M = fmaxf(M, f[w] = s_m[w][hh]);
 #pragma unroll
-                for (int w = 0; w < kWaves; w++) L += s_l[w][hh] * (mw[w] == M ? 1.f : __builtin_amdgcn_exp2f(mw[w] - M));
+                for (int w = 0; w < kWaves; w++) {
+                    f[w] = f[w] == M ? 1.f : __builtin_amdgcn_exp2f(f[w] - M);
+                    L = fmaf(s_l[w][hh], f[w], L);
+                }
 #pragma unroll
                 for (int e = 0; e < kVE; e++) o[e] = 0.f;
 #pragma unroll
@@ -630,7 +631,9 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
                     const int row = hh + k * GS;
                     const float *at = s_o + 256 * kVE * t + (row / 4 * 16 + (i & 15)) * 4 + row % 4;
 #pragma unroll
-                    for (int e = 0; e < kVE; e++) o[e] += at[256 * e] + at[kSum + 256 * e];
+                    for (int e = 0; e < kVE; e++)
+#pragma unroll
+                        for (int w = 0; w < kWaves; w++) o[e] = fmaf(at[w * kSum + 256 * e], f[w], o[e]);
                 }
 #pragma unroll
                 for (int e = 0; e < kVE; e++) z = fmaf(o[e] + L, 0.f, z);
