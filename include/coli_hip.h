@@ -369,7 +369,7 @@ int    coli_hip_pages_status(const ColiHipPages *p, int *n_free, int *errors, vo
  * the projection is gated: q_head = 2 hd, gate = q + hd); key head h at k + r * kv_row + h * hd,
  * the values alike. */
 typedef struct {
-    int H;                    /* query heads, a multiple of KH */
+    int H;                    /* query heads, a multiple of KH, at most 4096 */
     int rot;                  /* rotary columns, even, 0..hd */
     int interleaved;          /* pairs (2j, 2j + 1); 0: (j, j + rot / 2) */
     int64_t q_row, q_head, kv_row;
