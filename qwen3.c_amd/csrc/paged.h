@@ -52,6 +52,13 @@ __device__ __forceinline__ int row_pos(const PoolView &p, const int *seq, const 
     return at < -1 ? -2 : -3 - len;   // -2: no position; -3 - len: past the end
 }
 
+// Workgroup barrier for LDS alone: __syncthreads() also waits for every load in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // false, with a message, when the description is outside what the kernels take (host only)
 bool pool_view(const ColiHipPages *p, PoolView &v);
 // the stream of a call and whether it can run: device usable and current

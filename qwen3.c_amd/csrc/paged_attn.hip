@@ -373,6 +373,49 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
             }
         };
         fill(from, min(last - from, kWindow));
+        lds_barrier();
+        // a row that is always there, for the loads of keys that are not
+        long hot = 0;
+        v4u kb[kSub][kKC];
+        unsigned vb[kVK][kVS][kVW];
+        unsigned vm[kSub], vm_next[kSub];
+        auto load_k = [&](int i0) {
+#pragma unroll
+            for (int t = 0; t < kSub; t++) {
+                const long o = s_off[i0 + 16 * t + c];
+                vm_next[t] = (unsigned)__ballot(o >= 0) & 0xffffu;
+                const v4u *k = (const v4u *)(p.data + (o >= 0 ? o : hot));
+#pragma unroll
+                for (int i = 0; i < kKC; i++) {
+                    const int at = 4 * i + g;
+                    kb[t][i] = k[kExact || at * kKE < p.hd ? at : 0];
+                }
+            }
+        };
+        auto load_v = [&](int i0) {
+#pragma unroll
+            for (int j = 0; j < kVK; j++) {
+                const long o = s_off[i0 + 16 * (j / 4) + 4 * g + j % 4];
+                const char *v = p.data + p.kv_bytes + (o >= 0 ? o : hot);
+#pragma unroll
+                for (int i = 0; i < kVS; i++) {
+                    int d = (16 * i + c) * kVE;
+                    if (!kExact && d >= p.hd) d = 0;
+                    if (kVW == 4)
+                        *(uint4 *)vb[j][i] = *(const uint4 *)(v + d * (kWide ? 4 : 2));
+                    else
+                        *(uint2 *)vb[j][i] = *(const uint2 *)(v + d * (kWide ? 4 : 2));
+                }
+            }
+        };
+        auto start = [&] {   // the first tile of a window
+            hot = uniform(max(s_off[0], 0L));
+            load_k(wave * kTile);
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(wave * kTile);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        start();   // on their way while q is cut into its pieces
 #pragma unroll
         for (int k = 0; k < GS / kWaves; k++) {
             const int hh = wave + kWaves * k;
@@ -406,7 +449,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
                 }
             }
         }
-        __syncthreads();
+        lds_barrier();   // the loads stay in flight
         const float inv = T == COLI_HIP_F16 ? s_inv[c % GS] : 1.f;
 
         v4f acc[kVS][kVE];
@@ -419,48 +462,11 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         for (int w0 = from; w0 < last; w0 += kWindow) {
             const int nk = min(last - w0, kWindow);
             if (w0 != from) {
-                __syncthreads();
+                lds_barrier();
                 fill(w0, nk);
-                __syncthreads();
+                lds_barrier();
+                start();
             }
-            // a row that is always there, for the loads of keys that are not
-            const long hot = uniform(max(s_off[0], 0L));
-            v4u kb[kSub][kKC];
-            unsigned vb[kVK][kVS][kVW];
-            unsigned vm[kSub], vm_next[kSub];
-            auto load_k = [&](int i0) {
-#pragma unroll
-                for (int t = 0; t < kSub; t++) {
-                    const long o = s_off[i0 + 16 * t + c];
-                    vm_next[t] = (unsigned)__ballot(o >= 0) & 0xffffu;
-                    const v4u *k = (const v4u *)(p.data + (o >= 0 ? o : hot));
-#pragma unroll
-                    for (int i = 0; i < kKC; i++) {
-                        const int at = 4 * i + g;
-                        kb[t][i] = k[kExact || at * kKE < p.hd ? at : 0];
-                    }
-                }
-            };
-            auto load_v = [&](int i0) {
-#pragma unroll
-                for (int j = 0; j < kVK; j++) {
-                    const long o = s_off[i0 + 16 * (j / 4) + 4 * g + j % 4];
-                    const char *v = p.data + p.kv_bytes + (o >= 0 ? o : hot);
-#pragma unroll
-                    for (int i = 0; i < kVS; i++) {
-                        int d = (16 * i + c) * kVE;
-                        if (!kExact && d >= p.hd) d = 0;
-                        if (kVW == 4)
-                            *(uint4 *)vb[j][i] = *(const uint4 *)(v + d * (kWide ? 4 : 2));
-                        else
-                            *(uint2 *)vb[j][i] = *(const uint2 *)(v + d * (kWide ? 4 : 2));
-                    }
-                }
-            };
-            load_k(wave * kTile);
-            __builtin_amdgcn_sched_barrier(0);
-            load_v(wave * kTile);
-            __builtin_amdgcn_sched_barrier(0);
             for (int i0 = wave * kTile; i0 < nk; i0 += kKeys) {
                 unsigned all = 0xffffu;
 #pragma unroll
@@ -605,13 +611,13 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
             s_m[wave][c] = m;
             s_l[wave][c] = l;
         }
-        __syncthreads();
+        lds_barrier();   // the last loads, of no keys, need not have come
         float z = 0.f;   // NaN when a result of this thread's is not finite
         {
             float *so = s_o + wave * kSum + 4 * lane;
 #pragma unroll
             for (int t = 0; t < kVS * kVE; t++) *(v4f *)(so + 256 * t) = acc[t / kVE][t % kVE];
-            __syncthreads();
+            lds_barrier();
             // a thread: head hh's kVE columns from d0.  Rows of one head's pieces are GS apart.
             for (int i = tid; i < GS * kVS * 16; i += kThreads) {
                 const int hh = i / 16 % GS, t = i / 16 / GS, d0 = (16 * t + (i & 15)) * kVE;
