@@ -751,6 +751,47 @@ def test_captured_decode(mod, lib, dev):
     assert lib.pages_status(pools[0].c)[1] == 0
 
 
+def test_captured_pages(mod, lib, dev):
+    """Branches dropped, taken anew and grown, the pool closed up: captured once, replayed with other
+    lists in the same arrays and eager work between, against the model."""
+    pool = Pool(mod, lib, dev, F16, 2, 2, 32, 4, 50, 8, 10, seed=5)
+    m = Model(pool)
+    seq, cnt = ints([0, 1, 2, -1], dev), ints([9, 14, 4, 3], dev)
+    src, dst, one = ints([0, 1, 0], dev), ints([3, 4, 5], dev), ints([1, 0, 2], dev)
+
+    def lists(*pairs):
+        for t, v in pairs:
+            t.copy_(ints(v, dev))
+        torch.cuda.synchronize()
+
+    torch.cuda.synchronize()
+    lib.pages_append(pool.c, addr(seq), addr(cnt), 4)
+    m.append([0, 1, 2, -1], [9, 14, 4, 3])
+    m.check(pool, lib, "start")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        st = torch.cuda.current_stream().cuda_stream
+        lib.pages_free(pool.c, addr(dst), 3, st)
+        lib.pages_fork(pool.c, addr(src), addr(dst), 3, True, st)
+        lib.pages_append(pool.c, addr(dst), addr(one), 3, st)
+        lib.pages_compact(pool.c, st)
+    for a, b, c in (([0, 1, 0], [3, 4, 5], [1, 0, 2]), ([2, -1, 1], [5, 6, 3], [4, 1, 1]), ([1, 1, 1], [3, 4, 6], [2, 2, 2]),
+                    ([0, 2, 3], [5, 6, -1], [3, 0, 9]), ([5, 0, 0], [4, 3, 7], [1, 1, 1])):
+        lists((src, a), (dst, b), (one, c))
+        m.free(b)
+        m.fork(a, b, True)
+        m.append(b, c)
+        m.compact()
+        graph.replay()
+        torch.cuda.synchronize()
+        m.check(pool, lib, (a, b, c))
+        m.free([2])
+        lib.pages_free(pool.c, addr(x := ints([2], dev)), 1)   # eager work between
+        m.append([2], [6])
+        lib.pages_append(pool.c, addr(x2 := ints([2], dev)), addr(y := ints([6], dev)), 1)
+        m.check(pool, lib, "between")
+
+
 # ---------------------------------------------------------------- the layer block
 @pytest.mark.parametrize("dtype,n", [(F32, 1), (F32, 3), (F32, 6), (BF16, 5)], ids=lambda v: str(v))
 def test_gqa_paged_block(mod, lib, orc, gen, dev, dtype, n):
