@@ -41,9 +41,8 @@
 
 namespace coli {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves, kGroup = 16;   // kGroup: heads a wave takes
-constexpr int kMaxBlocks = 1024;
-constexpr int kWindow = 1024;   // keys whose row offsets a block holds in LDS at a time
+constexpr int kGroup = 16;        // heads a wave takes
+constexpr int kLaneRows = 8;      // rows of a lane while they are lined up: 512 rows or fewer
 constexpr float kLazy = 8.f;    // the maximum moves when a score passes it by 2^8: weights stay below
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -62,7 +61,7 @@ struct Cut {
     int block, slot;               // of its first part
 };
 
-// Keys of a wave's tile, and blocks that fit a CU by their registers.
+// Keys of a wave's tile, and waves that fit a SIMD by their registers.
 constexpr int tile_of(int T, int HD) { return T == COLI_HIP_F32 || HD == 256 ? 16 : 32; }
 constexpr int resident(int T, int HD) { return HD == 256 ? (T == COLI_HIP_F32 ? 1 : 2) : HD == 128 ? 2 : 4; }
 
@@ -72,6 +71,7 @@ struct PagedArgs {
     float *out, *part;
     float2 *ml;
     Cut *cut;
+    int stride;                  // heads of a part's place in the workspace
     int by_row;                  // cuts are listed by (row, kv head), else by the block they begin in
     int n, layer, groups, khv;   // head groups of kGroup per kv head, khv = KH * groups
     unsigned magic, shift;       // t / page = (umulhi(t, magic) + t) >> shift, t < 2^31
@@ -168,10 +168,10 @@ __device__ __forceinline__ float finish(float o, float l, int cnt, const float *
 
 // A part in plain fp32: keys [from, last) of the row, a key per wave at a time, four columns a
 // lane, head by head.
-template <int T>
+template <int T, int W>
 __device__ void slow_part(const PoolView &p, const HeadsView &h, const PagedArgs &a, int r, int s, int kh, long head,
                           int hn, int cnt, int from, int last, bool whole, long slot, float *s_o, float *s_ml) {
-    constexpr int kUp = Pieces<T>::up;
+    constexpr int kUp = Pieces<T>::up, kWaves = W;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = 4 * lane;
     const bool in = d0 < p.hd;
     const int *row = p.table + (size_t)s * p.max_pages;
@@ -211,25 +211,26 @@ __device__ void slow_part(const PoolView &p, const HeadsView &h, const PagedArgs
             f[w] = s_ml[2 * w] == M ? 1.f : __builtin_amdgcn_exp2f(s_ml[2 * w] - M);
             L += f[w] * s_ml[2 * w + 1];
         }
-        const int d = threadIdx.x;
-        if (d < p.hd) {
+        for (int d = threadIdx.x; d < p.hd; d += 64 * W) {
             float t = 0.f;
             for (int w = 0; w < kWaves; w++) t += f[w] * s_o[w * 256 + d];
             if (whole)
                 a.out[((long)r * h.H + head + hh) * p.hd + d] =
                     finish(t, L, cnt, a.gate, r * h.q_row + (head + hh) * h.q_head + d);
             else
-                a.part[(slot * kGroup + hh) * p.hd + d] = t;
+                a.part[(slot * a.stride + hh) * p.hd + d] = t;
         }
-        if (!whole && d == 0) a.ml[slot * kGroup + hh] = make_float2(M, L);
+        if (!whole && threadIdx.x == 0) a.ml[slot * a.stride + hh] = make_float2(M, L);
     }
     __syncthreads();
 }
 
 // HD: the head dim, or the next of 64, 128, 256 above it (kExact false).  GS: rows of a piece, at
-// least the heads of a group.
-template <int T, int HD, bool kExact, int GS>
-__global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView p, HeadsView h, PagedArgs a) {
+// least the heads of a group.  W: waves of a block.
+template <int T, int HD, bool kExact, int GS, int W>
+__global__ __launch_bounds__(64 * W, resident(T, HD)) void attn_part(PoolView p, HeadsView h, PagedArgs a) {
+    constexpr int kWaves = W, kThreads = 64 * W;
+    constexpr int kWindow = 256 * W - (W == 1 ? 128 : 0);   // keys whose row offsets are in LDS at a time
     constexpr bool kWide = T == COLI_HIP_F32;
     constexpr int kTile = tile_of(T, HD), kSub = kTile / 16, kKeys = kWaves * kTile;
     constexpr int kPieces = Pieces<T>::n, kUp = Pieces<T>::up, kNT = kWide ? 1 : (kPieces * GS + 15) / 16;
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
     constexpr int kQWords = kNT * 16 * kQRow, kOffWords = 2 * (kWindow + kPad), kSum = HD * 16;
     // q and the offsets of the keys' rows, then the waves' sums
     __shared__ __attribute__((aligned(16))) unsigned s_mem[kQWords + kOffWords > kWaves * kSum ? kQWords + kOffWords : kWaves * kSum];
-    __shared__ int s_cnt[kThreads], s_seq[kThreads], s_wave[kWaves], s_row, s_first;
+    __shared__ int s_cnt[64 * kLaneRows], s_wave[kWaves], s_row, s_first;
     __shared__ float s_inv[kGroup], s_m[kWaves][kGroup], s_l[kWaves][kGroup];
     unsigned *const s_q = s_mem;
     long *const s_off = (long *)(s_mem + kQWords);
@@ -250,19 +251,23 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 15, g = lane >> 4;
     const int G = h.H / p.KH;
 
-    // The units of all rows in one line: a thread has `per` rows; 64 rows or fewer every wave lines
-    // up for itself, a lane a row.
-    const bool few = a.n <= 64;
-    const int per = few ? 1 : (a.n + kThreads - 1) / kThreads, t0 = few ? lane : tid * per;
-    int mine = 0, total = 0, cnt_t = -1, seq_t = -1;
+    // The units of all rows in one line: a thread has `per` rows; up to 64 kLaneRows rows every wave
+    // lines up for itself.
+    auto units = [&](int cnt) { return units_of<kKeys, kSetup>(cnt) * a.khv; };
+    auto none = [&](int r) {   // no block has this row
+        if (a.by_row && !blockIdx.x)
+            for (int k = 0; k < a.khv; k++) a.cut[r * a.khv + k].parts = 0;
+    };
+    const bool few = a.n <= 64 * kLaneRows;
+    const int per = few ? (a.n + 63) / 64 : (a.n + kThreads - 1) / kThreads, t0 = (few ? lane : tid) * per;
+    int mine = 0, total = 0;
 #pragma unroll 4
     for (int i = 0; i < per; i++) {
-        const int r = t0 + i;
-        seq_t = -1;
-        cnt_t = r < a.n ? row_count(p, a, r, seq_t) : -1;
-        if (a.by_row && !blockIdx.x && r < a.n && cnt_t < 0)   // no block has this row
-            for (int k = 0; k < a.khv; k++) a.cut[r * a.khv + k].parts = 0;
-        mine += units_of<kKeys, kSetup>(cnt_t) * a.khv;
+        int s;
+        const int r = t0 + i, cnt = r < a.n ? row_count(p, a, r, s) : -1;
+        if (few) s_cnt[r] = cnt;   // every wave the same
+        if (r < a.n && cnt < 0) none(r);
+        mine += units(cnt);
     }
     int x = mine;
 #pragma unroll
@@ -271,11 +276,9 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         if (lane >= o) x += y;
     }
     int before = x - mine;
-    if (few) {
+    if (few || W == 1) {
         total = __builtin_amdgcn_readlane(x, 63);
     } else {
-        s_cnt[tid] = cnt_t;
-        s_seq[tid] = seq_t;
         if (lane == 63) s_wave[wave] = x;
         __syncthreads();
 #pragma unroll
@@ -292,19 +295,28 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         return;
     }
     // the row of unit u0, and the units before it
-    int r, first;
+    int r, first, s, cnt;
     const bool mine0 = before <= u0 && u0 < before + mine;
     if (few) {
-        r = __ffsll((unsigned long long)__ballot(mine0)) - 1;
-        first = __builtin_amdgcn_readlane(before, r);
+        const int l = __ffsll((unsigned long long)__ballot(mine0)) - 1;
+        r = l * per;
+        first = __builtin_amdgcn_readlane(before, l);
+        cnt = uniform(s_cnt[r]);
+        for (int i = 1; i < per; i++) {
+            const int k = units(cnt);
+            if (first + k > u0) break;
+            first += k;
+            cnt = uniform(s_cnt[++r]);
+        }
+        s = a.seq[r];
     } else {
         if (mine0) {
-            int k = tid * per;
+            int k = t0;
             for (int i = 1; i < per; i++) {
                 int s;
-                const int units = units_of<kKeys, kSetup>(row_count(p, a, k, s)) * a.khv;
-                if (before + units > u0) break;
-                before += units;
+                const int c = units(row_count(p, a, k, s));
+                if (before + c > u0) break;
+                before += c;
                 k++;
             }
             s_row = k;
@@ -313,27 +325,21 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         __syncthreads();
         r = uniform(s_row);
         first = uniform(s_first);
+        cnt = row_count(p, a, r, s);
     }
+    s = uniform(s);
+    cnt = uniform(cnt);
     Cut cut = {};
     int done = 0;   // whether the block has had a part before
 
-    for (int u = u0; u < end && r < a.n;) {
-        int s, cnt;
-        if (few) {
-            s = __builtin_amdgcn_readlane(seq_t, r);
-            cnt = __builtin_amdgcn_readlane(cnt_t, r);
-        } else if (per == 1) {
-            s = uniform(s_seq[r]);
-            cnt = uniform(s_cnt[r]);
-        } else {
-            cnt = uniform(row_count(p, a, r, s));
-            s = uniform(s);
-        }
+    for (int u = u0; u < end;) {
         const int nc = chunks_of<kKeys>(cnt), nu = units_of<kKeys, kSetup>(cnt);
         const int xx = u - first;
         if (xx >= nu * a.khv) {   // this row is done (or has none)
             first += nu * a.khv;
-            r++;
+            if (++r >= a.n) break;
+            cnt = uniform(few ? s_cnt[r] : row_count(p, a, r, s));
+            s = uniform(a.seq[r]);
             continue;
         }
         const int hv = uniform((int)((unsigned)xx / (unsigned)nu)), x0 = xx - hv * nu;
@@ -643,14 +649,14 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
                 }
 #pragma unroll
                 for (int e = 0; e < kVE; e++) z = fmaf(o[e] + L, 0.f, z);
-                float *dst = a.part + (slot * kGroup + hh) * p.hd + d0;
+                float *dst = a.part + (slot * a.stride + hh) * p.hd + d0;
                 if (whole) {
                     dst = a.out + ((long)r * h.H + head + hh) * p.hd + d0;
                     const long gat = r * h.q_row + (head + hh) * h.q_head + d0;
 #pragma unroll
                     for (int e = 0; e < kVE; e++) o[e] = finish(o[e], L, cnt, a.gate, gat + e);
                 } else if (d0 == 0) {
-                    a.ml[slot * kGroup + hh] = make_float2(M, L);
+                    a.ml[slot * a.stride + hh] = make_float2(M, L);
                 }
 #pragma unroll
                 for (int e = 0; e < kVE; e += 4) *(float4 *)(dst + e) = *(const float4 *)(o + e);
@@ -658,7 +664,7 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
         }
         // the sums' place is the next part's q; 16-bit products that met an infinity or NaN: again
         if (__syncthreads_or(!kWide && z != 0.f))
-            slow_part<T>(p, h, a, r, s, kh, head, hn, cnt, from, last, whole, slot, s_o, &s_m[0][0]);
+            slow_part<T, W>(p, h, a, r, s, kh, head, hn, cnt, from, last, whole, slot, s_o, &s_m[0][0]);
         if (c0 == 0) {   // u is behind its unit c1
             cut = Cut{};
             if (c1 < nc) {
@@ -674,16 +680,17 @@ __global__ __launch_bounds__(kThreads, resident(T, HD)) void attn_part(PoolView 
 
 // Block (i, hh, z): columns z * cols.. of head hh of cut i.  A thread has four columns of every
 // ks-th part; the first kAhead parts are on their way while the weights are found.
-constexpr int kAhead = 8;
-__global__ __launch_bounds__(kThreads) void attn_join(PoolView p, HeadsView h, PagedArgs a, int cols) {
-    __shared__ float s_w[kMaxBlocks], s_red[kWaves];
-    __shared__ v4f s_o[kThreads];
+constexpr int kAhead = 8, kJoin = 256;
+constexpr int kJoinW = 1024;   // parts whose weights are kept; of more they are taken again
+__global__ __launch_bounds__(kJoin) void attn_join(PoolView p, HeadsView h, PagedArgs a, int cols) {
+    __shared__ float s_w[kJoinW], s_red[kJoin / 64];
+    __shared__ v4f s_o[kJoin];
     const Cut cut = a.cut[blockIdx.x];
     const int hh = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = cut.parts;
     if (!n || hh >= cut.heads) return;
-    const int wide = cols / 4, d = blockIdx.z * cols + tid % wide * 4, k0 = tid / wide, ks = kThreads / wide;
+    const int wide = cols / 4, d = blockIdx.z * cols + tid % wide * 4, k0 = tid / wide, ks = kJoin / wide;
     const bool in = d < p.hd;
-    auto at = [&](int k) { return (k ? 2L * (cut.block + k) : (long)cut.slot) * kGroup + hh; };
+    auto at = [&](int k) { return (k ? 2L * (cut.block + k) : (long)cut.slot) * a.stride + hh; };
     v4f x[kAhead], o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < kAhead; j++) {
@@ -691,10 +698,9 @@ __global__ __launch_bounds__(kThreads) void attn_join(PoolView p, HeadsView h, P
         x[j] = k < n && in ? *(const v4f *)(a.part + at(k) * p.hd + d) : o;
     }
     float m = -INFINITY, l = 0.f;
-    for (int k = tid; k < n; k += kThreads) {
+    for (int k = tid; k < n; k += kJoin) {
         const float2 ml = a.ml[at(k)];
         m = fmaxf(m, ml.x);
-        s_w[k] = ml.x;
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
@@ -702,10 +708,11 @@ __global__ __launch_bounds__(kThreads) void attn_join(PoolView p, HeadsView h, P
     __syncthreads();
     m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
     __syncthreads();
-    for (int k = tid; k < n; k += kThreads) {
-        const float f = s_w[k] == m ? 1.f : __builtin_amdgcn_exp2f(s_w[k] - m);
-        s_w[k] = f;
-        l += f * a.ml[at(k)].y;
+    for (int k = tid; k < n; k += kJoin) {
+        const float2 ml = a.ml[at(k)];
+        const float f = ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
+        if (k < kJoinW) s_w[k] = f;
+        l += f * ml.y;
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
@@ -719,7 +726,11 @@ __global__ __launch_bounds__(kThreads) void attn_join(PoolView p, HeadsView h, P
     }
     if (in) {
 #pragma unroll 8
-        for (int k = k0 + kAhead * ks; k < n; k += ks) o += s_w[k] * *(const v4f *)(a.part + at(k) * p.hd + d);
+        for (int k = k0 + kAhead * ks; k < min(n, kJoinW); k += ks) o += s_w[k] * *(const v4f *)(a.part + at(k) * p.hd + d);
+        for (int k = kJoinW + k0; k < n; k += ks) {
+            const float x = a.ml[at(k)].x, f = x == m ? 1.f : __builtin_amdgcn_exp2f(x - m);
+            o += f * *(const v4f *)(a.part + at(k) * p.hd + d);
+        }
     }
     s_o[tid] = o;
     __syncthreads();
@@ -731,50 +742,79 @@ __global__ __launch_bounds__(kThreads) void attn_join(PoolView p, HeadsView h, P
 }
 
 // Blocks of a launch: all of them resident, so that equal shares end together.
-static int max_blocks(int T, int hd) { return 256 * resident(T, hd <= 64 ? 64 : hd <= 128 ? 128 : 256); }
+static int max_blocks(int T, int HD, int W) { return 256 * resident(T, HD) * (4 / W); }
+static int head_dim(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
-size_t attn_paged_work(const PoolView &p) {
-    const size_t b = max_blocks(p.es == 4 ? COLI_HIP_F32 : COLI_HIP_F16, p.hd);
-    return 2 * b * kGroup * (p.hd * sizeof(float) + sizeof(float2)) + b * sizeof(Cut);
+// Blocks of one wave (heads of up to 128 only) where a wave has a (row, kv head) to itself rather
+// than four waves a short one each: from kMany of them, of kShort keys or fewer.  16-bit pages, 8 kv
+// heads of 128, ragged, us with 1 / 4 waves: 64 rows of up to 300 keys 18 / 21, 128 of 300 23 / 28,
+// 256 of 32 15 / 28, 500 of 300 54 / 74, 128 of 1200 36 / 37; but 32 of 128 14 / 12, and heads of 256
+// 128 rows of 300 27 / 22.
+constexpr int kShort = 1024, kMany = 512;
+static int waves_of(int HD, long row_heads, int max_len) {
+    return HD <= 128 && max_len > 0 && max_len <= kShort && row_heads >= kMany ? 1 : 4;
 }
 
-template <int T, int GS>
+// Two parts a block, each of up to 16 heads.
+size_t attn_paged_work(const PoolView &p) {
+    const int T = p.es == 4 ? COLI_HIP_F32 : COLI_HIP_F16, HD = head_dim(p.hd);
+    const size_t blocks = max_blocks(T, HD, HD <= 128 ? 1 : 4);
+    return 2 * blocks * kGroup * (p.hd * sizeof(float) + sizeof(float2)) + blocks * sizeof(Cut);
+}
+
+template <int T, int GS, int W>
 static void launch(const PoolView &pv, const HeadsView &hv, const PagedArgs &a, int blocks, hipStream_t st) {
-    const dim3 g(blocks), t(kThreads);
+    const dim3 g(blocks), t(64 * W);
     switch (pv.hd) {
-    case 64: hipLaunchKernelGGL((attn_part<T, 64, true, GS>), g, t, 0, st, pv, hv, a); return;
-    case 128: hipLaunchKernelGGL((attn_part<T, 128, true, GS>), g, t, 0, st, pv, hv, a); return;
-    case 256: hipLaunchKernelGGL((attn_part<T, 256, true, GS>), g, t, 0, st, pv, hv, a); return;
+    case 64: hipLaunchKernelGGL((attn_part<T, 64, true, GS, W>), g, t, 0, st, pv, hv, a); return;
+    case 128: hipLaunchKernelGGL((attn_part<T, 128, true, GS, W>), g, t, 0, st, pv, hv, a); return;
+    }
+    if constexpr (W == 4) {
+        if (pv.hd == 256) {
+            hipLaunchKernelGGL((attn_part<T, 256, true, GS, W>), g, t, 0, st, pv, hv, a);
+            return;
+        }
+        if (pv.hd > 128) {
+            hipLaunchKernelGGL((attn_part<T, 256, false, GS, W>), g, t, 0, st, pv, hv, a);
+            return;
+        }
     }
     if (pv.hd < 64)
-        hipLaunchKernelGGL((attn_part<T, 64, false, GS>), g, t, 0, st, pv, hv, a);
-    else if (pv.hd < 128)
-        hipLaunchKernelGGL((attn_part<T, 128, false, GS>), g, t, 0, st, pv, hv, a);
+        hipLaunchKernelGGL((attn_part<T, 64, false, GS, W>), g, t, 0, st, pv, hv, a);
     else
-        hipLaunchKernelGGL((attn_part<T, 256, false, GS>), g, t, 0, st, pv, hv, a);
+        hipLaunchKernelGGL((attn_part<T, 128, false, GS, W>), g, t, 0, st, pv, hv, a);
 }
 
-template <int T>
+template <int T, int W>
 static void launch_heads(const PoolView &pv, const HeadsView &hv, const PagedArgs &a, int blocks, hipStream_t st) {
-    const int G = hv.H / pv.KH;
-    if (G <= 4)
-        launch<T, 4>(pv, hv, a, blocks, st);
-    else if (G <= 8)
-        launch<T, 8>(pv, hv, a, blocks, st);
-    else
-        launch<T, 16>(pv, hv, a, blocks, st);
+    if constexpr (T != COLI_HIP_F32) {
+        if (a.stride == 8) return launch<T, 8, W>(pv, hv, a, blocks, st);
+        if (a.stride == 4) return launch<T, 4, W>(pv, hv, a, blocks, st);
+    }
+    launch<T, 16, W>(pv, hv, a, blocks, st);
+}
+
+template <int W>
+static void launch_type(const PoolView &pv, const HeadsView &hv, int dtype, const PagedArgs &a, int blocks, hipStream_t st) {
+    switch (dtype) {
+    case COLI_HIP_F32: launch_heads<COLI_HIP_F32, W>(pv, hv, a, blocks, st); break;
+    case COLI_HIP_F16: launch_heads<COLI_HIP_F16, W>(pv, hv, a, blocks, st); break;
+    default: launch_heads<COLI_HIP_BF16, W>(pv, hv, a, blocks, st);
+    }
 }
 
 bool attn_paged(const PoolView &pv, const HeadsView &hv, int dtype, int layer, const float *q, const float *gate,
                 const int *seq, const int *pos, int n, int max_len, float *out, void *work, hipStream_t st) {
-    const int most = max_blocks(dtype, pv.hd), G = hv.H / pv.KH;
-    const int keys = kWaves * tile_of(dtype, pv.hd <= 64 ? 64 : pv.hd <= 128 ? 128 : 256);
+    const int G = hv.H / pv.KH, HD = head_dim(pv.hd), GS = dtype == COLI_HIP_F32 || G > 8 ? 16 : G > 4 ? 8 : 4;
+    const int groups = (G + kGroup - 1) / kGroup, W = waves_of(HD, (long)n * pv.KH * groups, max_len);
+    const int most = max_blocks(dtype, HD, W), keys = W * tile_of(dtype, HD);
     PagedArgs a;
     a.q = q, a.gate = gate, a.seq = seq, a.pos = pos, a.out = out, a.n = n, a.layer = layer;
     a.part = (float *)work;
-    a.ml = (float2 *)(a.part + 2 * (size_t)most * kGroup * pv.hd);
-    a.cut = (Cut *)(a.ml + 2 * (size_t)most * kGroup);
-    a.groups = (G + kGroup - 1) / kGroup;
+    a.ml = (float2 *)(a.part + 2 * (size_t)most * GS * pv.hd);
+    a.cut = (Cut *)(a.ml + 2 * (size_t)most * GS);
+    a.stride = GS;
+    a.groups = groups;
     a.khv = pv.KH * a.groups;
     a.shift = 0;
     while ((1L << a.shift) < pv.page) a.shift++;
@@ -789,16 +829,15 @@ bool attn_paged(const PoolView &pv, const HeadsView &hv, int dtype, int layer, c
         const long units = ((len + keys - 1) / keys) * a.khv * (long)a.n;   // more blocks would cut setups only
         const int blocks = (int)(units < most ? units : most);
         a.by_row = a.n * (long)a.khv <= blocks;
-        switch (dtype) {
-        case COLI_HIP_F32: launch<COLI_HIP_F32, 16>(pv, hv, a, blocks, st); break;
-        case COLI_HIP_F16: launch_heads<COLI_HIP_F16>(pv, hv, a, blocks, st); break;
-        default: launch_heads<COLI_HIP_BF16>(pv, hv, a, blocks, st);
-        }
+        if (W == 1)
+            launch_type<1>(pv, hv, dtype, a, blocks, st);
+        else
+            launch_type<4>(pv, hv, dtype, a, blocks, st);
         if (blocks > 1) {
             // few cuts: blocks of 64 columns (16 parts at a time); else of a whole head
             const int cuts = a.by_row ? a.n * a.khv : blocks, heads = G < kGroup ? G : kGroup;
             const int cols = cuts * heads <= 512 ? 64 : pv.hd <= 64 ? 64 : pv.hd <= 128 ? 128 : 256;
-            hipLaunchKernelGGL(attn_join, dim3(cuts, heads, (pv.hd + cols - 1) / cols), dim3(kThreads), 0, st, pv, hv, a,
+            hipLaunchKernelGGL(attn_join, dim3(cuts, heads, (pv.hd + cols - 1) / cols), dim3(kJoin), 0, st, pv, hv, a,
                                cols);
         }
         a.q += (size_t)a.n * hv.H * pv.hd;

@@ -464,6 +464,39 @@ def test_attn_many_rows(mod, lib, dev, dtype, KH, hd, n):
     assert bool((got[rest] == torch.tensor([77.0 if seq[i] < 0 else 0.0 for i in rest])[:, None, None]).all())
 
 
+@pytest.mark.parametrize("dtype,H,KH,hd,n,page", [
+    (BF16, 32, 8, 128, 80, 16), (F16, 8, 8, 64, 70, 5), (F32, 16, 8, 128, 64, 32), (BF16, 18, 1, 80, 600, 16),
+    (F16, 4, 4, 8, 130, 1), (F32, 6, 2, 72, 270, 16), (F16, 24, 4, 112, 128, 64), (BF16, 7, 1, 64, 513, 24),
+], ids=lambda v: str(v))
+def test_attn_short_and_many(mod, lib, dev, dtype, H, KH, hd, n, page):
+    """Many short rows, for which a (row, kv head) takes one wave: a length as long as the hint, one
+    far past it, none at all, rows of no sequence; the same rows without a hint agree, and where an
+    infinity or NaN is seen they agree on that."""
+    rng = np.random.default_rng(n)
+    lens = [int(x) for x in rng.integers(1, 90, 30)] + [0, 1, 1000, 3500]
+    pool = Pool(mod, lib, dev, dtype, 1, KH, hd, page, sum(-(-x // page) for x in lens) + 1, len(lens),
+                -(-3500 // page), seed=3)
+    pool.place(lens)
+    a = Attn(mod, lib, dev, pool, H, n % 2 == 0, seed=1)
+    seq = [int(x) for x in rng.integers(-1, len(lens), n)]
+    seq[:4], seq[-2:] = [-1, 33, 32, 31], [30, -1]
+    counts = [lens[s] if s >= 0 else 0 for s in seq]
+    q, raw = a.rows(n)
+    got = a.run(q, raw, seq, max_len=1000)
+    assert lib.pages_status(pool.c)[1] == 0
+    check = sorted(set(range(0, n, max(1, n // 60))) | {0, 1, 2, 3, n - 2, n - 1})
+    a.check(got[check], q[check], raw[check], [seq[i] for i in check], [counts[i] for i in check])
+    free = a.run(q, raw, seq)
+    assert torch.allclose(got, free, rtol=1e-4, atol=1e-5)
+    assert torch.equal(got, a.run(q, raw, seq, max_len=1000))
+    for s, kv, x in ((3, 1, float("inf")), (33, 0, float("nan")), (32, 1, float("-inf"))):
+        pool.data[pool.table[s, 0].long(), 0, kv, 0, 0, 5] = x
+    torch.cuda.synchronize()
+    got, free = a.run(q, raw, seq, max_len=1000), a.run(q, raw, seq)
+    assert not bool(torch.isfinite(got).all())
+    assert torch.allclose(got, free, rtol=1e-4, atol=1e-5, equal_nan=True)
+
+
 def test_offsets_past_32_bits(mod, lib, dev):
     """A pool of 6.5 GB whose sequence lies at its far end: rows written, attended, copied there and
     moved down from there."""
