@@ -26,15 +26,15 @@
 // Work: a unit is kKeys keys (a tile per wave) of a kv head, 64 KB or so; a (row, kv head) counts
 // kSetup units more, about what its q, row offsets and sums cost beside the keys (200 ragged rows of
 // 45 to 2900 keys, 8 kv heads: 156 us without, 125 with one).  The units of all rows in one line
-// are cut into equal shares, one per block, whatever the lengths are.  A (row, kv head) that a
-// border cuts goes through the workspace, and attn_join joins its parts.
+// are cut into equal shares, one per block (of four waves, or of one for many short rows), whatever
+// the lengths are.  A (row, kv head) that a border cuts goes through the workspace, and attn_join
+// joins its parts.
 //
 // Bound by the bytes of K and V where there are many: two rows of 120000 keys (2 kv heads of 256,
-// f16) 98 us, 5.0 TB/s (a large copy here moves 4.9); 48 rows of up to 16000 keys 70 us, 4.3; the 200
-// rows above 125 us, 4.6.  Bound by a chain of latencies where there are few: one row of 600 keys
-// 15 us, of which 4 are the join.  Tried and left out: 32-key tiles for heads of 256 (spills: 48 rows
-// 121 us against 78), more blocks per CU for heads of 128 (154 us with two, 165 with three), a join
-// by the last block to arrive (its fences and atomics take as long as the second launch).
+// f16) 97 us, 5.1 TB/s (a large copy here moves 4.9); 48 rows of up to 16000 keys 68 us, 4.4; the 200
+// rows above 124 us, 4.6.  Bound by a chain of latencies where there are few: one row of 600 keys
+// 14 us, of which 4 are the join.  Tried and left out: 32-key tiles for heads of 256 (spills: 48 rows
+// 121 us against 78), more blocks per CU for heads of 128 (154 us with two, 165 with three).
 #include "paged.h"
 
 #include <math.h>
@@ -43,7 +43,7 @@ namespace coli {
 
 constexpr int kGroup = 16;        // heads a wave takes
 constexpr int kLaneRows = 8;      // rows of a lane while they are lined up: 512 rows or fewer
-constexpr float kLazy = 8.f;    // the maximum moves when a score passes it by 2^8: weights stay below
+constexpr float kLazy = 8.f;      // the maximum moves when a score passes it by 2^8: weights stay below
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -746,10 +746,10 @@ static int max_blocks(int T, int HD, int W) { return 256 * resident(T, HD) * (4 
 static int head_dim(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
 // Blocks of one wave (heads of up to 128 only) where a wave has a (row, kv head) to itself rather
-// than four waves a short one each: from kMany of them, of kShort keys or fewer.  16-bit pages, 8 kv
-// heads of 128, ragged, us with 1 / 4 waves: 64 rows of up to 300 keys 18 / 21, 128 of 300 23 / 28,
-// 256 of 32 15 / 28, 500 of 300 54 / 74, 128 of 1200 36 / 37; but 32 of 128 14 / 12, and heads of 256
-// 128 rows of 300 27 / 22.
+// than four waves a short one each: from kMany of them, of kShort keys or fewer.  bf16 pages, 8 kv
+// heads of 128, ragged, us with 1 / 4 waves: 64 rows of up to 300 keys 18 / 21, 128 of 300 22 / 28,
+// 256 of 32 15 / 28, 500 of 300 54 / 74, 128 of 1200 36 / 37; but 32 of 128 14 / 12, and 128 rows of 300
+// with 2 kv heads of 256 27 / 22.
 constexpr int kShort = 1024, kMany = 512;
 static int waves_of(int HD, long row_heads, int max_len) {
     return HD <= 128 && max_len > 0 && max_len <= kShort && row_heads >= kMany ? 1 : 4;
