@@ -384,7 +384,8 @@ int    coli_hip_heads_check(const ColiHipPages *p, const ColiHipHeads *h);
  * lens - 1): queries normed and rotated into d_qout [n][H][hd], keys normed, rotated and rounded
  * into the sequence's page of the layer, values rounded beside them.  The position must be held
  * already (append first): a row past the end, or with sequence -1, is skipped whole.  Two rows
- * with one position leave either's K and V.  Angles are pos * freq in 64 bits. */
+ * with one position leave either's K and V.  Angles are pos * freq in 64 bits.  d_qout overlaps no
+ * input. */
 int    coli_hip_qk_rope_paged(const ColiHipPages *p, const ColiHipHeads *h, int layer, const float *d_q,
                               const float *d_k, const float *d_v, const int *d_seq, const int *d_pos, int n,
                               float *d_qout, void *stream);
@@ -393,7 +394,9 @@ int    coli_hip_qk_rope_paged(const ColiHipPages *p, const ColiHipHeads *h, int 
  * (strides q_row, q_head).  d_q is [n][H][hd] as qk_rope leaves it.  A row that sees no position
  * gives 0; a row with sequence -1 is left as it was; one past the end sees what the sequence
  * holds.  max_len: the longest sequence in the call as far as the caller knows (0: unknown); only the split
- * of the work goes by it.  d_out and d_work are aligned to 16 bytes;
+ * of the work goes by it.  Sums of values times weights are held in fp32 before they are divided
+ * by the weights' sum: values past 2^88 in magnitude may give infinities.  d_out overlaps no
+ * input; d_out and d_work are aligned to 16 bytes;
  * d_work: coli_hip_attn_paged_work() bytes, not shared by calls that may run at once, no contents kept. */
 size_t coli_hip_attn_paged_work(const ColiHipPages *p, const ColiHipHeads *h);
 int    coli_hip_attn_paged(const ColiHipPages *p, const ColiHipHeads *h, int layer, const float *d_q,
@@ -402,7 +405,7 @@ int    coli_hip_attn_paged(const ColiHipPages *p, const ColiHipHeads *h, int lay
 /* An attention layer of n rows of many sequences, the batch form of coli_vk_gqa_full on device
  * rows: d_x [n][D] (normed) -> q (| gate where gq_t has 2 H hd rows), k, v -> qk_rope into the
  * pages -> attention -> out_t -> d_out [n][out_t rows].  The positions must have been appended.
- * A row with sequence -1 gives 0.  The strides of h are not used.  Shares the layer blocks'
+ * A row with sequence -1, or past its sequence's end, gives 0.  The strides of h are not used.  Shares the layer blocks'
  * scratch: one stream, and not one that is being captured. */
 int    coli_hip_gqa_paged(const ColiHipPages *p, const ColiHipHeads *h, int layer, const float *d_x, int D,
                           const ColiVkTensor *gq_t, const ColiVkTensor *gk_t, const ColiVkTensor *gv_t,

@@ -59,6 +59,12 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// What the wave's lanes wrote to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // false, with a message, when the description is outside what the kernels take (host only)
 bool pool_view(const ColiHipPages *p, PoolView &v);
 // the stream of a call and whether it can run: device usable and current

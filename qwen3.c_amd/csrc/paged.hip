@@ -16,6 +16,8 @@ static bool heads_view(const ColiHipPages *p, const ColiHipHeads *h, HeadsView &
     if (h->H < 1 || h->H % p->KH || h->H > 4096) return paged_refuse("query heads not a multiple of the kv heads");
     if (h->rot < 0 || h->rot > p->hd || h->rot % 2) return paged_refuse("rotary columns not even, or more than a head");
     if (h->rot && !h->freq) return paged_refuse("NULL inverse frequencies");
+    constexpr int64_t kFar = (int64_t)1 << 40;   // times rows or heads: within 63 bits
+    if (h->q_head > kFar || h->q_row > kFar || h->kv_row > kFar) return paged_refuse("row stride past 2^40");
     if (h->q_head < p->hd || h->q_row < (h->H - 1) * h->q_head + p->hd || h->kv_row < (int64_t)p->KH * p->hd)
         return paged_refuse("rows that overlap");
     v.H = h->H, v.rot = h->rot, v.interleaved = h->interleaved != 0;
@@ -109,7 +111,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void qk_rope_rows(PoolView p, Head
         sincospif((float)(2.0 * a), &sn, &cs);
         s_turn[wave][lane + 64 * i] = make_float2(cs * h.mag, sn * h.mag);
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     float cs[4], sn[4];
     bool second[4];
 #pragma unroll
@@ -143,13 +145,13 @@ __global__ __launch_bounds__(64 * kRopeWaves) void qk_rope_rows(PoolView p, Head
         } else if (h.rot) {   // the other half's columns are other lanes' of this wave
             float *row = s_x[wave] + sub * 4 * LP;
             *(v4f *)(row + d0) = y;
-            __builtin_amdgcn_wave_barrier();
+            wave_sync();
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int d = d0 + i;
                 if (d < h.rot) o[i] = y[i] * cs[i] + row[second[i] ? d - hr : d + hr] * sn[i];
             }
-            __builtin_amdgcn_wave_barrier();
+            wave_sync();
         }
         if (isv) o = x;
         if (live && isq) {
@@ -197,7 +199,7 @@ static bool rope_launch(const PoolView &pv, const HeadsView &hv, int dtype, int 
 }
 
 // ---------------------------------------------------------------- the layer block
-enum { P_Q, P_K, P_V, P_QN, P_CTX, P_WORK, P_COUNT };
+enum { P_Q, P_K, P_V, P_QN, P_CTX, P_SEQ, P_WORK, P_COUNT };
 static struct {
     void *p = nullptr;
     size_t cap = 0;
@@ -207,9 +209,16 @@ void paged_shutdown() {
     for (auto &w : g_pw) scratch_free(&w.p, &w.cap);
 }
 
-__global__ __launch_bounds__(256) void fill_zero(float *x, size_t n) {
+// The context cleared (nc floats), and the rows that attend: those at a position which is held, so
+// that the rotation has written their query; others get sequence -1 and keep the zeros.
+__global__ __launch_bounds__(256) void block_rows(PoolView p, const int *__restrict__ seq, const int *__restrict__ pos,
+                                                  int n, int *__restrict__ live, float *__restrict__ ctx, size_t nc) {
     const size_t i = blockIdx.x * (size_t)256 + threadIdx.x;
-    if (i < n) x[i] = 0.f;
+    if (i < nc) ctx[i] = 0.f;
+    if (i < (size_t)n) {
+        int s;
+        live[i] = row_pos(p, seq, pos, (int)i, s) < 0 ? -1 : s;
+    }
 }
 
 }  // namespace coli
@@ -280,18 +289,19 @@ COLI_API int coli_hip_gqa_paged(const ColiHipPages *p, const ColiHipHeads *h, in
     if (hipStreamIsCapturing(st, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone)
         return paged_refuse("the layer block in a captured stream (its scratch may grow)") ? 1 : 0;
     const size_t rows = n, need[P_COUNT] = {rows * gq_t->O * 4,       rows * KH * hd * 4,     rows * KH * hd * 4,
-                                            rows * h->H * hd * 4,     rows * h->H * hd * 4,
+                                            rows * h->H * hd * 4,     rows * h->H * hd * 4,   rows * 4,
                                             coli_hip_attn_paged_work(p, &own)};
     for (int i = 0; i < P_COUNT; i++)
         if (!scratch(&g_pw[i].p, &g_pw[i].cap, need[i])) return 0;
     float *q = (float *)g_pw[P_Q].p, *k = (float *)g_pw[P_K].p, *v = (float *)g_pw[P_V].p;
     float *qn = (float *)g_pw[P_QN].p, *ctx = (float *)g_pw[P_CTX].p;
     if (!gemv(gq_t, d_x, q, n, st) || !gemv(gk_t, d_x, k, n, st) || !gemv(gv_t, d_x, v, n, st)) return 0;
-    // a row without a sequence: no attention writes its context
-    const size_t nc = rows * h->H * hd;
-    hipLaunchKernelGGL(fill_zero, dim3((unsigned)((nc + 255) / 256)), dim3(256), 0, st, ctx, nc);
+    int *live = (int *)g_pw[P_SEQ].p;
+    const size_t nc = rows * h->H * hd;   // more than the rows
+    hipLaunchKernelGGL(block_rows, dim3((unsigned)((nc + 255) / 256)), dim3(256), 0, st, pv, d_seq, d_pos, n, live, ctx,
+                       nc);
     if (!rope_launch(pv, hv, p->dtype, layer, q, k, v, d_seq, d_pos, n, qn, st) ||
-        !attn_paged(pv, hv, p->dtype, layer, qn, gated ? q + hd : nullptr, d_seq, d_pos, n, max_len, ctx,
+        !attn_paged(pv, hv, p->dtype, layer, qn, gated ? q + hd : nullptr, live, d_pos, n, max_len, ctx,
                      g_pw[P_WORK].p, st))
         return 0;
     return gemv(out_t, ctx, d_out, n, st) ? 1 : 0;

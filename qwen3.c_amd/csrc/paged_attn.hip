@@ -238,6 +238,7 @@ __global__ __launch_bounds__(64 * W, resident(T, HD)) void attn_part(PoolView p,
     constexpr int kVE = HD >= 16 * kKE ? kKE : HD / 16, kVS = HD / (16 * kVE);     // V alike
     constexpr int kVW = kWide ? kVE : kVE / 2, kVK = kTile / 4;                    // words of a V piece, keys of a lane
     constexpr int kUnit = kKeys * HD * (kWide ? 8 : 4), kSetup = kUnit >= 65536 ? 1 : 65536 / kUnit;
+    static_assert(kSetup <= 8, "the host counts a row's units with 8");
     constexpr int kPad = kKeys + kTile;                                            // offsets read past the last key
     constexpr int kQRow = kWide ? HD + 4 : HD / 2 + 4;                             // words of a q row in LDS
     constexpr int kQWords = kNT * 16 * kQRow, kOffWords = 2 * (kWindow + kPad), kSum = HD * 16;
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(64 * W, resident(T, HD)) void attn_part(PoolView p,
         const int *row = p.table + (size_t)s * p.max_pages;
         const long fix = a.layer * p.layer_bytes + kh * p.head_bytes;
 
-        // q in units of log 2, in pieces; a wave takes every fourth head
+        // q in units of log 2, in pieces; a wave takes every W-th head
         float qx[GS / kWaves][HD / 64];
 #pragma unroll
         for (int k = 0; k < GS / kWaves; k++)
@@ -821,7 +822,7 @@ bool attn_paged(const PoolView &pv, const HeadsView &hv, int dtype, int layer, c
     a.magic = (unsigned)(((1ULL << 32) * ((1ULL << a.shift) - pv.page)) / pv.page + 1);
     const long cap = (long)pv.max_pages * pv.page, len = max_len > 0 && max_len < cap ? max_len : cap;
     // the units of a launch's rows are counted in 31 bits: more rows go in several launches
-    const long row = ((cap + keys - 1) / keys + 4) * a.khv;
+    const long row = ((cap + keys - 1) / keys + 8) * a.khv;   // kSetup is 8 at most
     if (row >= 1L << 30) return paged_refuse("a sequence of more than 2^30 units");
     const int rows = (int)min((long)n, (1L << 30) / row);
     for (int r = 0; r < n; r += rows) {

@@ -910,3 +910,36 @@ def test_gqa_paged_matches_dense(mod, lib, gen, dev):
         args = list(ok)
         args[i] = v
         assert L.coli_hip_gqa_paged(*args) == 0, i
+
+
+def test_gqa_paged_rows_past_the_end(mod, lib, gen, dev):
+    """A row whose position is not held has no query: the block gives 0 for it, whatever an earlier
+    call left in its scratch, and the other rows are as without it."""
+    D, H, KH, hd, rot, gs = 256, 4, 2, 64, 16, 128
+    W = _layers.GqaWeights(gen, gen.stream(0x9E00, 1), D, H, KH, hd, rot, gs)
+    tq, tk, tv, to = (m.upload(lib) for m in (W.q, W.k, W.v, W.o))
+    pool = Pool(mod, lib, dev, BF16, 1, KH, hd, 4, 12, 3, 4, seed=2)
+    freq = torch.tensor([float(np.float32(float(W.theta) ** (-2.0 * j / rot))) for j in range(rot // 2)], device=dev)
+    heads = mod.Lib.heads(H=H, rot=rot, interleaved=0, q_row=2 * H * hd, q_head=2 * hd, kv_row=KH * hd, eps=1e-6,
+                          rope_mag=1.0, scale=1.0 / math.sqrt(hd), freq=addr(freq))
+    x = torch.from_numpy(np.concatenate([gen.normal(D, 0x9E10 + t) for t in range(4)])).to(dev)
+
+    def go(pos):
+        s, p, out = ints([0, 1, 0, 2], dev), ints(pos, dev), torch.full((4, D), 4.0, device=dev)
+        torch.cuda.synchronize()
+        lib.gqa_paged_dev(pool.c, heads, 0, addr(x), tq, tk, tv, to, addr(s), addr(p), 4, 6, addr(out))
+        sync(lib)
+        return out, lib.pages_status(pool.c)[1]
+
+    lens, cnt = ints([0, 1], dev), ints([5, 6], dev)
+    torch.cuda.synchronize()
+    lib.pages_append(pool.c, addr(lens), addr(cnt), 2)
+    for t in range(5):   # every position written; the scratch holds queries of all rows
+        go([t, t, t, -1])
+    go([4, 5, 3, -1])
+    whole, err = go([4, 5, 4, -1])
+    assert err == 0 and bool(whole[:3].any(1).all()) and not bool(whole[3].any())
+    for pos, bit in (([4, 5, 5, -1], 16), ([4, 5, 2 ** 31 - 1, 0], 16), ([4, 5, -2, -1], 4)):
+        out, err = go(pos)
+        assert err == bit and not bool(out[2:].any()), pos
+        assert torch.equal(out[1], whole[1]), pos

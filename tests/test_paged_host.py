@@ -77,3 +77,11 @@ def test_no_device_no_work(mod, bare):
     assert L.coli_hip_qk_rope_paged(p, h, 0, a, a, a, a, None, 2, a, None) == 0
     assert L.coli_hip_attn_paged(p, h, 0, a, None, a, None, 2, 0, a, a, 1 << 30, None) == 0
     assert L.coli_hip_gqa_paged(p, h, 0, a, 64, None, None, None, None, a, None, 2, 0, a, None) == 0
+
+
+@pytest.mark.parametrize("change", [dict(q_row=(1 << 40) + 1), dict(q_head=1 << 60, q_row=1 << 62),
+                                    dict(kv_row=1 << 62)], ids=str)
+def test_refused_far_strides(mod, bare, change):
+    """Offsets of a call's rows stay within 64 bits."""
+    p, h = mod.Lib.pages(**GOOD), mod.Lib.heads(**dict(HEADS, **change))
+    assert bare.L.coli_hip_heads_check(C.byref(p), C.byref(h)) == 0
