@@ -394,7 +394,7 @@ int    coli_hip_qk_rope_paged(const ColiHipPages *p, const ColiHipHeads *h, int 
  * (strides q_row, q_head).  d_q is [n][H][hd] as qk_rope leaves it.  A row that sees no position
  * gives 0; a row with sequence -1 is left as it was; one past the end sees what the sequence
  * holds.  max_len: the longest sequence in the call as far as the caller knows (0: unknown); only the split
- * of the work goes by it.  Sums of values times weights are held in fp32 before they are divided
+ * of the work goes by it (short rows take one launch instead of two).  Sums of values times weights are held in fp32 before they are divided
  * by the weights' sum: values past 2^88 in magnitude may give infinities.  d_out overlaps no
  * input; d_out and d_work are aligned to 16 bytes;
  * d_work: coli_hip_attn_paged_work() bytes, not shared by calls that may run at once, no contents kept. */

@@ -26,9 +26,10 @@
 // Work: a unit is kKeys keys (a tile per wave) of a kv head, 64 KB or so; a (row, kv head) counts
 // kSetup units more, about what its q, row offsets and sums cost beside the keys (200 ragged rows of
 // 45 to 2900 keys, 8 kv heads: 156 us without, 125 with one).  The units of all rows in one line
-// are cut into equal shares, one per block (of four waves, or of one for many short rows), whatever
-// the lengths are.  A (row, kv head) that a border cuts goes through the workspace, and attn_join
-// joins its parts.
+// are cut into equal shares, one per block of four waves, whatever the lengths are.  A (row, kv head)
+// that a border cuts goes through the workspace, and attn_join joins its parts.  Where the caller says
+// that the rows are short, each (row, kv head) is a block's instead, of four waves or of one (whole_by):
+// no lining up, no second launch.
 //
 // Bound by the bytes of K and V where there are many: two rows of 120000 keys (2 kv heads of 256,
 // f16) 97 us, 5.1 TB/s (a large copy here moves 4.9); 48 rows of up to 16000 keys 68 us, 4.4; the 200
@@ -72,6 +73,7 @@ struct PagedArgs {
     float2 *ml;
     Cut *cut;
     int stride;                  // heads of a part's place in the workspace
+    int direct;                  // block (row, kv head) has all of it: no units, no cuts (always with W 1)
     int by_row;                  // cuts are listed by (row, kv head), else by the block they begin in
     int n, layer, groups, khv;   // head groups of kGroup per kv head, khv = KH * groups
     unsigned magic, shift;       // t / page = (umulhi(t, magic) + t) >> shift, t < 2^31
@@ -230,7 +232,7 @@ __device__ void slow_part(const PoolView &p, const HeadsView &h, const PagedArgs
 template <int T, int HD, bool kExact, int GS, int W>
 __global__ __launch_bounds__(64 * W, resident(T, HD)) void attn_part(PoolView p, HeadsView h, PagedArgs a) {
     constexpr int kWaves = W, kThreads = 64 * W;
-    constexpr int kWindow = 256 * W - (W == 1 ? 128 : 0);   // keys whose row offsets are in LDS at a time
+    constexpr int kWindow = W == 1 ? 128 : 1024;   // keys whose row offsets are in LDS at a time
     constexpr bool kWide = T == COLI_HIP_F32;
     constexpr int kTile = tile_of(T, HD), kSub = kTile / 16, kKeys = kWaves * kTile;
     constexpr int kPieces = Pieces<T>::n, kUp = Pieces<T>::up, kNT = kWide ? 1 : (kPieces * GS + 15) / 16;
@@ -259,7 +261,15 @@ __global__ __launch_bounds__(64 * W, resident(T, HD)) void attn_part(PoolView p,
         if (a.by_row && !blockIdx.x)
             for (int k = 0; k < a.khv; k++) a.cut[r * a.khv + k].parts = 0;
     };
-    const bool few = a.n <= 64 * kLaneRows;
+    const bool direct = W == 1 || a.direct, few = !direct && a.n <= 64 * kLaneRows;
+    int r, first, s, cnt, u0, end, share = 1;
+    if (direct) {
+        r = uniform((int)(blockIdx.x / (unsigned)a.khv));
+        cnt = row_count(p, a, r, s);
+        if (cnt < 0) return;
+        const int nu = units_of<kKeys, kSetup>(cnt);
+        first = 0, u0 = ((int)blockIdx.x - r * a.khv) * nu, end = u0 + nu;
+    } else {
     const int per = few ? (a.n + 63) / 64 : (a.n + kThreads - 1) / kThreads, t0 = (few ? lane : tid) * per;
     int mine = 0, total = 0;
 #pragma unroll 4
@@ -277,7 +287,7 @@ __global__ __launch_bounds__(64 * W, resident(T, HD)) void attn_part(PoolView p,
         if (lane >= o) x += y;
     }
     int before = x - mine;
-    if (few || W == 1) {
+    if (few) {
         total = __builtin_amdgcn_readlane(x, 63);
     } else {
         if (lane == 63) s_wave[wave] = x;
@@ -289,14 +299,13 @@ __global__ __launch_bounds__(64 * W, resident(T, HD)) void attn_part(PoolView p,
         }
         total = uniform(total);
     }
-    const int share = uniform((int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
-    const int u0 = min(total, (int)blockIdx.x * share), end = min(total, u0 + share);
+    share = uniform((int)((unsigned)(total + gridDim.x - 1) / gridDim.x));
+    u0 = min(total, (int)blockIdx.x * share), end = min(total, u0 + share);
     if (u0 >= end) {
         if (tid == 0 && !a.by_row) a.cut[blockIdx.x].parts = 0;
         return;
     }
     // the row of unit u0, and the units before it
-    int r, first, s, cnt;
     const bool mine0 = before <= u0 && u0 < before + mine;
     if (few) {
         const int l = __ffsll((unsigned long long)__ballot(mine0)) - 1;
@@ -327,6 +336,7 @@ __global__ __launch_bounds__(64 * W, resident(T, HD)) void attn_part(PoolView p,
         r = uniform(s_row);
         first = uniform(s_first);
         cnt = row_count(p, a, r, s);
+    }
     }
     s = uniform(s);
     cnt = uniform(cnt);
@@ -666,7 +676,7 @@ __global__ __launch_bounds__(64 * W, resident(T, HD)) void attn_part(PoolView p,
         // the sums' place is the next part's q; 16-bit products that met an infinity or NaN: again
         if (__syncthreads_or(!kWide && z != 0.f))
             slow_part<T, W>(p, h, a, r, s, kh, head, hn, cnt, from, last, whole, slot, s_o, &s_m[0][0]);
-        if (c0 == 0) {   // u is behind its unit c1
+        if (c0 == 0 && !direct) {   // u is behind its unit c1
             cut = Cut{};
             if (c1 < nc) {
                 const int parts = (int)((unsigned)(u + (nc - c1) - 1) / (unsigned)share) - (int)blockIdx.x + 1;
@@ -676,7 +686,7 @@ __global__ __launch_bounds__(64 * W, resident(T, HD)) void attn_part(PoolView p,
         }
         done = 1;
     }
-    if (tid == 0 && !a.by_row) a.cut[blockIdx.x] = cut;   // only the last part can go on
+    if (tid == 0 && !direct && !a.by_row) a.cut[blockIdx.x] = cut;   // only the last part can go on
 }
 
 // Block (i, hh, z): columns z * cols.. of head hh of cut i.  A thread has four columns of every
@@ -743,23 +753,33 @@ __global__ __launch_bounds__(kJoin) void attn_join(PoolView p, HeadsView h, Page
 }
 
 // Blocks of a launch: all of them resident, so that equal shares end together.
-static int max_blocks(int T, int HD, int W) { return 256 * resident(T, HD) * (4 / W); }
+static int max_blocks(int T, int HD) { return 256 * resident(T, HD); }
 static int head_dim(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
-// Blocks of one wave (heads of up to 128 only) where a wave has a (row, kv head) to itself rather
-// than four waves a short one each: from kMany of them, of kShort keys or fewer.  bf16 pages, 8 kv
-// heads of 128, ragged, us with 1 / 4 waves: 64 rows of up to 300 keys 18 / 21, 128 of 300 22 / 28,
-// 256 of 32 15 / 28, 500 of 300 54 / 74, 128 of 1200 36 / 37; but 32 of 128 14 / 12, and 128 rows of 300
-// with 2 kv heads of 256 27 / 22.
-constexpr int kShort = 1024, kMany = 512;
-static int waves_of(int HD, long row_heads, int max_len) {
-    return HD <= 128 && max_len > 0 && max_len <= kShort && row_heads >= kMany ? 1 : 4;
+// Waves of the blocks where each has a (row, kv head) to itself, or 0: units in equal shares.  us
+// with whole rows / shares, ragged rows of up to so many keys:
+//   few (row, kv head)s, up to 300 KB of K and V each; kv heads of 256, bf16: one row of 128 keys
+//   10.6 / 16.3, 300 14.4 / 15, 600 20 / 15; 8 heads of 128: 128 7.6 / 10.6, 600 11.8 / 13.3, 1200 18.5 / 13.3;
+//   8 of 64, f32: 300 9.6 / 12.6, 600 13.9 / 12.6
+//   from 128 on, where shares are cut oftener, up to 450 KB; 128 rows, 2 kv heads of 256: 300 15.8 / 22, 600
+//   21.5 / 23.4, 1200 33.5 / 31; 8 of 128, f32: 300 29.6 / 33.9, 1200 74 / 64
+//   from 512 on up to 640 KB; 2 kv heads of 256, 260 to 400 rows of 600 all alike 79 to 107 / 85 to 117, ragged
+//   28 to 45 / 35 to 56; 8 of 128, 65 and 150 rows of 1200 74, 133 / 74, 146, ragged 30, 57 / 27, 58
+// One wave instead of four where not all blocks of four are resident and the rows are short for that (us
+// with 1 / 4; 8 heads of 128, bf16: 128 rows of 128 10 / 16.7, 600 27.7 / 25.3; 500 of 300 42 / 68; f32: 128 of 32
+// 10 / 16.6, 300 36 / 29.6; 500 rows, 2 heads of 256: 128 25.8 / 26.2, 300 39 / 34), and, 16 bits and heads up to 128,
+// for rows of a tile (6.5 / 7.5).
+static int whole_by(int T, int HD, long row_heads, int max_len) {
+    const long bytes = 2L * max_len * HD * (T == COLI_HIP_F32 ? 4 : 2), blocks = max_blocks(T, HD);
+    if (max_len <= 0 || bytes > (row_heads < 128 ? 300L : row_heads < 512 ? 450L : 640L) << 10) return 0;
+    if (T != COLI_HIP_F32 && HD <= 128 && max_len <= tile_of(T, HD)) return 1;
+    return row_heads > blocks && max_len * blocks <= 5 * tile_of(T, HD) * row_heads ? 1 : 4;
 }
 
 // Two parts a block, each of up to 16 heads.
 size_t attn_paged_work(const PoolView &p) {
     const int T = p.es == 4 ? COLI_HIP_F32 : COLI_HIP_F16, HD = head_dim(p.hd);
-    const size_t blocks = max_blocks(T, HD, HD <= 128 ? 1 : 4);
+    const size_t blocks = max_blocks(T, HD);
     return 2 * blocks * kGroup * (p.hd * sizeof(float) + sizeof(float2)) + blocks * sizeof(Cut);
 }
 
@@ -769,21 +789,14 @@ static void launch(const PoolView &pv, const HeadsView &hv, const PagedArgs &a, 
     switch (pv.hd) {
     case 64: hipLaunchKernelGGL((attn_part<T, 64, true, GS, W>), g, t, 0, st, pv, hv, a); return;
     case 128: hipLaunchKernelGGL((attn_part<T, 128, true, GS, W>), g, t, 0, st, pv, hv, a); return;
-    }
-    if constexpr (W == 4) {
-        if (pv.hd == 256) {
-            hipLaunchKernelGGL((attn_part<T, 256, true, GS, W>), g, t, 0, st, pv, hv, a);
-            return;
-        }
-        if (pv.hd > 128) {
-            hipLaunchKernelGGL((attn_part<T, 256, false, GS, W>), g, t, 0, st, pv, hv, a);
-            return;
-        }
+    case 256: hipLaunchKernelGGL((attn_part<T, 256, true, GS, W>), g, t, 0, st, pv, hv, a); return;
     }
     if (pv.hd < 64)
         hipLaunchKernelGGL((attn_part<T, 64, false, GS, W>), g, t, 0, st, pv, hv, a);
-    else
+    else if (pv.hd < 128)
         hipLaunchKernelGGL((attn_part<T, 128, false, GS, W>), g, t, 0, st, pv, hv, a);
+    else
+        hipLaunchKernelGGL((attn_part<T, 256, false, GS, W>), g, t, 0, st, pv, hv, a);
 }
 
 template <int T, int W>
@@ -807,8 +820,7 @@ static void launch_type(const PoolView &pv, const HeadsView &hv, int dtype, cons
 bool attn_paged(const PoolView &pv, const HeadsView &hv, int dtype, int layer, const float *q, const float *gate,
                 const int *seq, const int *pos, int n, int max_len, float *out, void *work, hipStream_t st) {
     const int G = hv.H / pv.KH, HD = head_dim(pv.hd), GS = dtype == COLI_HIP_F32 || G > 8 ? 16 : G > 4 ? 8 : 4;
-    const int groups = (G + kGroup - 1) / kGroup, W = waves_of(HD, (long)n * pv.KH * groups, max_len);
-    const int most = max_blocks(dtype, HD, W), keys = W * tile_of(dtype, HD);
+    const int most = max_blocks(dtype, HD), keys = 4 * tile_of(dtype, HD), groups = (G + kGroup - 1) / kGroup;
     PagedArgs a;
     a.q = q, a.gate = gate, a.seq = seq, a.pos = pos, a.out = out, a.n = n, a.layer = layer;
     a.part = (float *)work;
@@ -824,16 +836,24 @@ bool attn_paged(const PoolView &pv, const HeadsView &hv, int dtype, int layer, c
     // the units of a launch's rows are counted in 31 bits: more rows go in several launches
     const long row = ((cap + keys - 1) / keys + 8) * a.khv;   // kSetup is 8 at most
     if (row >= 1L << 30) return paged_refuse("a sequence of more than 2^30 units");
+    const long row_heads = (long)n * a.khv;
+    const int whole = row < 1L << 28 && row_heads <= 1L << 22 ? whole_by(dtype, HD, row_heads, max_len) : 0;
+    a.direct = whole != 0;
+    if (whole) {
+        a.n = n;
+        if (whole == 1)
+            launch_type<1>(pv, hv, dtype, a, (int)row_heads, st);
+        else
+            launch_type<4>(pv, hv, dtype, a, (int)row_heads, st);
+        return paged_launched("paged attention launch");
+    }
     const int rows = (int)min((long)n, (1L << 30) / row);
     for (int r = 0; r < n; r += rows) {
         a.n = min(rows, n - r);
         const long units = ((len + keys - 1) / keys) * a.khv * (long)a.n;   // more blocks would cut setups only
         const int blocks = (int)(units < most ? units : most);
         a.by_row = a.n * (long)a.khv <= blocks;
-        if (W == 1)
-            launch_type<1>(pv, hv, dtype, a, blocks, st);
-        else
-            launch_type<4>(pv, hv, dtype, a, blocks, st);
+        launch_type<4>(pv, hv, dtype, a, blocks, st);
         if (blocks > 1) {
             // few cuts: blocks of 64 columns (16 parts at a time); else of a whole head
             const int cuts = a.by_row ? a.n * a.khv : blocks, heads = G < kGroup ? G : kGroup;

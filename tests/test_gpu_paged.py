@@ -469,7 +469,7 @@ def test_attn_many_rows(mod, lib, dev, dtype, KH, hd, n):
     (F16, 4, 4, 8, 130, 1), (F32, 6, 2, 72, 270, 16), (F16, 24, 4, 112, 128, 64), (BF16, 7, 1, 64, 513, 24),
 ], ids=lambda v: str(v))
 def test_attn_short_and_many(mod, lib, dev, dtype, H, KH, hd, n, page):
-    """Many short rows, for which a (row, kv head) takes one wave: a length as long as the hint, one
+    """Many short rows: a length as long as the hint, one
     far past it, none at all, rows of no sequence; the same rows without a hint agree, and where an
     infinity or NaN is seen they agree on that."""
     rng = np.random.default_rng(n)
@@ -495,6 +495,50 @@ def test_attn_short_and_many(mod, lib, dev, dtype, H, KH, hd, n, page):
     got, free = a.run(q, raw, seq, max_len=1000), a.run(q, raw, seq)
     assert not bool(torch.isfinite(got).all())
     assert torch.allclose(got, free, rtol=1e-4, atol=1e-5, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype,H,KH,hd,n,page,hints", [
+    (BF16, 32, 8, 128, 90, 16, (5, 40, 200, 0)), (BF16, 16, 2, 256, 300, 16, (40, 90, 200)),
+    (F16, 8, 8, 64, 150, 5, (30, 60, 500)), (F32, 16, 8, 128, 80, 32, (9, 33, 150)), (BF16, 18, 1, 80, 600, 16, (8, 50, 64)),
+    (F16, 4, 4, 8, 300, 1, (16, 33, 300)), (F32, 6, 2, 72, 270, 16, (12, 70)), (F16, 24, 4, 112, 140, 64, (64, 150)),
+    (BF16, 7, 1, 64, 1100, 24, (32, 33, 1000)), (F32, 5, 5, 256, 60, 8, (20, 140)), (F16, 40, 2, 200, 280, 16, (31, 99)),
+    (F32, 8, 8, 48, 140, 16, (16, 17, 300)), (BF16, 2, 1, 136, 3, 16, (1, 30)), (F16, 20, 1, 128, 1, 16, (1, 90)),
+], ids=lambda v: str(v))
+def test_attn_whole_rows(mod, lib, dev, dtype, H, KH, hd, n, page, hints):
+    """Hints small enough that a block of one wave or of four has a (row, kv head) to itself: lengths
+    up to the hint, none, one far past it; rows of no sequence; infinities and NaN."""
+    for hint in hints:
+        rng = np.random.default_rng(1000 * n + hint)
+        top = max(hint, 1)
+        lens = [int(x) for x in rng.integers(0, top + 1, 20)] + [top, 0, 1, max(1, top - 1), 1500]
+        pool = Pool(mod, lib, dev, dtype, 2, KH, hd, page, sum(-(-x // page) for x in lens) + 1, len(lens),
+                    -(-1500 // page), seed=hint)
+        pool.place(lens)
+        a = Attn(mod, lib, dev, pool, H, n % 2 == 0, seed=1)
+        seq = [int(x) for x in rng.integers(-1, len(lens), n)]
+        seq[0] = 20
+        if n > 8:
+            seq[1:5], seq[-2:] = [-1, 24, 21, 22], [23, -1]
+        counts = [lens[s] if s >= 0 else 0 for s in seq]
+        q, raw = a.rows(n)
+        got = a.run(q, raw, seq, max_len=hint)
+        assert lib.pages_status(pool.c)[1] == 0
+        check = sorted(set(range(0, n, max(1, n // 40))) | set(range(min(n, 5))) | {n - 1, max(0, n - 2)})
+        a.check(got[check], q[check], raw[check], [seq[i] for i in check], [counts[i] for i in check])
+        none = [i for i in range(n) if seq[i] < 0]
+        assert bool((got[none] == 77.0).all())
+        assert torch.equal(got, a.run(q, raw, seq, max_len=hint))
+        if hint:
+            few = min(n, 3)
+            some = a.run(q[:few].contiguous(), raw[:few].contiguous(), seq[:few], max_len=hint)
+            assert torch.allclose(some, got[:few], rtol=1e-4, atol=1e-5)
+        for s, kv, x in ((20, 1, float("inf")), (22, 0, float("nan"))):
+            if lens[s]:
+                pool.data[pool.table[s, 0].long(), 0, kv, 0, 0, 5] = x
+        torch.cuda.synchronize()
+        got, free = a.run(q, raw, seq, max_len=hint), a.run(q, raw, seq)
+        assert not bool(torch.isfinite(got[0]).all())
+        assert torch.allclose(got, free, rtol=1e-4, atol=1e-5, equal_nan=True)
 
 
 def test_offsets_past_32_bits(mod, lib, dev):
