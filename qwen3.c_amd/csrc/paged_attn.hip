@@ -62,9 +62,13 @@ struct Cut {
     int block, slot;               // of its first part
 };
 
-// Keys of a wave's tile, and waves that fit a SIMD by their registers.
+// Keys of a wave's tile, and waves that fit a SIMD by their registers.  Four for 16-bit heads of 64 spill: 32
+// ragged rows of 2400 keys, 8 kv heads, 22.1 us with four, 17.0 with three; blocks of one wave keep four
+// (500 rows of 32: 11.7 / 12.5).
 constexpr int tile_of(int T, int HD) { return T == COLI_HIP_F32 || HD == 256 ? 16 : 32; }
-constexpr int resident(int T, int HD) { return HD == 256 ? (T == COLI_HIP_F32 ? 1 : 2) : HD == 128 ? 2 : 4; }
+constexpr int resident(int T, int HD, int W = 4) {
+    return HD == 256 ? (T == COLI_HIP_F32 ? 1 : 2) : HD == 128 ? 2 : T == COLI_HIP_F32 || W == 1 ? 4 : 3;
+}
 
 struct PagedArgs {
     const float *q, *gate;
@@ -236,7 +240,7 @@ __device__ void slow_part(const PoolView &p, const HeadsView &h, const PagedArgs
 // HD: the head dim, or the next of 64, 128, 256 above it (kExact false).  GS: rows of a piece, at
 // least the heads of a group.  W: waves of a block.
 template <int T, int HD, bool kExact, int GS, int W>
-__global__ __launch_bounds__(64 * W, resident(T, HD)) void attn_part(PoolView p, HeadsView h, PagedArgs a) {
+__global__ __launch_bounds__(64 * W, resident(T, HD, W)) void attn_part(PoolView p, HeadsView h, PagedArgs a) {
     constexpr int kWaves = W, kThreads = 64 * W;
     constexpr int kWindow = W == 1 ? 128 : 1024;   // keys whose row offsets are in LDS at a time
     constexpr bool kWide = T == COLI_HIP_F32;
