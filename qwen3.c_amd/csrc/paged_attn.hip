@@ -33,8 +33,8 @@
 //
 // Bound by the bytes of K and V where there are many: two rows of 120000 keys (2 kv heads of 256,
 // f16) 97 us, 5.1 TB/s (a large copy here moves 4.9); 48 rows of up to 16000 keys 68 us, 4.4; the 200
-// rows above 124 us, 4.6.  Bound by a chain of latencies where there are few: one row of 600 keys
-// 14 us, of which 4 are the join.  Tried and left out: 32-key tiles for heads of 256 (spills: 48 rows
+// rows above 121 us, 4.7.  Bound by a chain of latencies where there are few: one row of 600 keys
+// 15 us, of which 4 are the join; one of 8 keys, whole, 8.4.  Tried and left out: 32-key tiles for heads of 256 (spills: 48 rows
 // 121 us against 78), more blocks per CU for heads of 128 (154 us with two, 165 with three).
 #include "paged.h"
 
