@@ -34,8 +34,9 @@
 // Bound by the bytes of K and V where there are many: two rows of 120000 keys (2 kv heads of 256,
 // f16) 97 us, 5.1 TB/s (a large copy here moves 4.9); 48 rows of up to 16000 keys 68 us, 4.4; the 200
 // rows above 121 us, 4.7.  Bound by a chain of latencies where there are few: one row of 600 keys
-// 15 us, of which 4 are the join; one of 8 keys, whole, 8.4.  Tried and left out: 32-key tiles for heads of 256 (spills: 48 rows
-// 121 us against 78), more blocks per CU for heads of 128 (154 us with two, 165 with three).
+// 15 us, of which 4 are the join; one of 8 keys, whole, 8.4.  Tried and left out: 32-key tiles for
+// heads of 256 (spills: 48 rows 121 us against 78), more blocks per CU for heads of 128 (154 us with two,
+// 165 with three), blocks of eight waves for whole rows (one row of 600 keys 19.8 us with four, 21.5).
 #include "paged.h"
 
 #include <math.h>
@@ -768,19 +769,19 @@ __global__ __launch_bounds__(kJoin) void attn_join(PoolView p, HeadsView h, Page
 static int max_blocks(int T, int HD) { return 256 * resident(T, HD); }
 static int head_dim(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
-// Waves of the blocks where each has a (row, kv head) to itself, or 0: units in equal shares.  us
-// with whole rows / shares, ragged rows of up to so many keys:
-//   few (row, kv head)s, up to 300 KB of K and V each; kv heads of 256, bf16: one row of 128 keys
-//   10.6 / 16.3, 300 14.4 / 15, 600 20 / 15; 8 heads of 128: 128 7.6 / 10.6, 600 11.8 / 13.3, 1200 18.5 / 13.3;
-//   8 of 64, f32: 300 9.6 / 12.6, 600 13.9 / 12.6
-//   from 128 on, where shares are cut oftener, up to 450 KB; 128 rows, 2 kv heads of 256: 300 15.8 / 22, 600
-//   21.5 / 23.4, 1200 33.5 / 31; 8 of 128, f32: 300 29.6 / 33.9, 1200 74 / 64
-//   from 512 on up to 640 KB; 2 kv heads of 256, 260 to 400 rows of 600 all alike 79 to 107 / 85 to 117, ragged
-//   28 to 45 / 35 to 56; 8 of 128, 65 and 150 rows of 1200 74, 133 / 74, 146, ragged 30, 57 / 27, 58
+// Waves of the blocks where each has a (row, kv head) to itself, or 0: units in equal shares.  us with
+// whole rows / shares, ragged rows of up to so many keys where there are several:
+//   few (row, kv head)s, up to 300 KB of K and V each; 2 kv heads of 256, bf16: one row of 128 keys 9.9 / 15.5,
+//   300 13.7 / 14.7, 600 19.5 / 14.8; 8 of 128: 128 7.3 / 10.3, 600 11.7 / 13.4, 1200 18.5 / 13.4; 8 of 64, f32:
+//   300 9.9 / 12.5, 600 14.2 / 12.6
+//   from 128 on, where shares are cut oftener, up to 450 KB; 128 rows, 2 kv heads of 256: 300 15.9 / 20.8, 600
+//   22.1 / 22.0, 1200 35 / 27; 8 of 128, f32: 300 30.5 / 32.8, 1200 77 / 63
+//   from 512 on up to 640 KB; 2 kv heads of 256, 260 to 400 rows of 600 all alike 79 to 105 / 83 to 116, ragged
+//   27 to 42 / 33 to 49; 8 of 128, 65 and 150 rows of 1200 75, 136 / 73, 145, ragged 29, 54 / 26, 56
 // One wave instead of four where not all blocks of four are resident and the rows are short for that (us
-// with 1 / 4; 8 heads of 128, bf16: 128 rows of 128 10 / 16.7, 600 27.7 / 25.3; 500 of 300 42 / 68; f32: 128 of 32
-// 10 / 16.6, 300 36 / 29.6; 500 rows, 2 heads of 256: 128 25.8 / 26.2, 300 39 / 34), and, 16 bits and heads up to 128,
-// for rows of a tile (6.5 / 7.5).
+// with 1 / 4; 8 heads of 128, bf16: 128 rows of 128 10 / 15.6, 600 27.4 / 23.7; 500 of 300 42 / 65; f32: 128 of 32
+// 9.8 / 16.4, 300 34 / 30.5; 500 rows, 2 heads of 256: 128 22.9 / 24.4, 300 36 / 32), and, 16 bits and heads up to
+// 128, for rows of a tile (6.3 / 7.0).
 static int whole_by(int T, int HD, long row_heads, int max_len) {
     const long bytes = 2L * max_len * HD * (T == COLI_HIP_F32 ? 4 : 2), blocks = max_blocks(T, HD);
     if (max_len <= 0 || bytes > (row_heads < 128 ? 300L : row_heads < 512 ? 450L : 640L) << 10) return 0;
