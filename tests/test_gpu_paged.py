@@ -987,3 +987,48 @@ def test_gqa_paged_rows_past_the_end(mod, lib, gen, dev):
         out, err = go(pos)
         assert err == bit and not bool(out[2:].any()), pos
         assert torch.equal(out[1], whole[1]), pos
+
+
+@pytest.mark.parametrize("hint", [8, 40])   # a block of one wave, and of four, has a row
+def test_captured_whole_rows(mod, lib, dev, hint):
+    """Two captured steps with a hint, over one workspace, replayed while the sequences grow past
+    the hint and rows come and go: every replay against the same call run eagerly."""
+    H, KH, hd, n = 8, 2, 64, 4
+    pool = Pool(mod, lib, dev, F16, 1, KH, hd, 4, 120, n, 30, seed=5)
+    att = Attn(mod, lib, dev, pool, H, True, seed=6)
+    lens, seq = ints([3, 0, 9, 30], dev), ints([0, 1, -1, 3], dev)
+    every, more = ints(range(n), dev), ints([7, 0, 9, 11], dev)
+    torch.cuda.synchronize()
+    lib.pages_append(pool.c, addr(every), addr(lens), n)
+    lib.sync()
+    q, raw = (t.to(dev) for t in att.rows(n))
+    out = [torch.full((n, H, hd), 5.0, device=dev) for _ in range(3)]
+
+    def step(o, st):
+        lib.attn_paged_dev(pool.c, att.heads, 0, addr(q), addr(raw) + 4 * hd, addr(seq), None, n, hint, addr(o),
+                           addr(att.work), att.work.numel(), st)
+
+    step(out[2], None)
+    lib.sync()
+    side = torch.cuda.Stream()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for i, graph in enumerate(graphs):
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            step(out[i], torch.cuda.current_stream().cuda_stream)
+    for t in range(5):
+        for o in out:
+            o.fill_(5.0)
+        torch.cuda.synchronize()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        step(out[2], None)
+        lib.sync()
+        assert torch.equal(out[0], out[2]) and torch.equal(out[1], out[2]), t
+        att.check(torch.where(out[2] == 5.0, 77.0, out[2]).cpu(), q.cpu(), raw.cpu(), seq.tolist(),
+                  [int(pool.lens[s]) if s >= 0 else 0 for s in seq.tolist()])
+        lib.pages_append(pool.c, addr(every), addr(more), n)
+        lib.sync()
+        seq.copy_(ints([0, 1, 2, 3] if t % 2 else [3, -1, 0, 2], dev))
+    assert lib.pages_status(pool.c)[1] == 0
