@@ -314,7 +314,7 @@ int   coli_hip_gdn_chunked(int on);
  *   refs  [n_pages] table entries that hold the page (0: free)
  *   used  [ceil(n_pages / 32)] bitmap of pages in use (bit p % 32 of word p / 32)
  *   state [COLI_HIP_PAGES_STATE] error bits and words of the library
- *   work  [coli_hip_pages_work()] ints of scratch, no contents kept between calls
+ *   work  [coli_hip_pages_work()] ints of the library, of one pool alone
  * All arrays are the caller's device memory; coli_hip_pages_init fills the bookkeeping ones
  * (not data).  hd is a multiple of 8 in 8..256, page 1..4096, max_pages * page at most 2^30.
  * The functions read and change the arrays on the device, in stream order, with no host
@@ -335,14 +335,16 @@ typedef struct {
 /* 1 when the description is one the library takes (host only, no device needed), else 0 with a
  * message.  Every function below checks it as well.  Rows of a call: at most 2^20. */
 int    coli_hip_pages_check(const ColiHipPages *p);
-/* ints that `work` has to hold. */
+/* ints that `work` has to hold (n_pages and n_seqs of the description are read). */
 size_t coli_hip_pages_work(const ColiHipPages *p);
 /* An empty pool: every page free, every sequence of length 0. */
 int    coli_hip_pages_init(const ColiHipPages *p, void *stream);
 /* Sequence d_seq[i] grows by d_count[i] >= 0 positions (d_count NULL: 1), n <= 4096.  New pages
  * are taken lowest free page first, in the order of the list; the new positions' K and V are
  * whatever the pages hold until qk_rope writes them.  All or nothing: when pages or a table row
- * do not suffice, or a sequence is named twice, nothing changes and an error bit is set. */
+ * do not suffice, or a sequence is named twice, nothing changes and an error bit is set; the
+ * sequences that were to grow have no new position then, and qk_rope without d_pos skips them until
+ * one of them grows, is freed or is forked into. */
 int    coli_hip_pages_append(const ColiHipPages *p, const int *d_seq, const int *d_count, int n, void *stream);
 /* Sequence d_dst[i], which must be empty, becomes a copy of d_src[i] (a pair with a -1 is
  * skipped), n <= 4096.  share != 0: full pages are shared (their counts grow), the last, partly
@@ -360,7 +362,8 @@ int    coli_hip_pages_compact(const ColiHipPages *p, void *stream);
 /* Waits for the stream; the number of free pages and the error bits gathered since the last
  * call (cleared by it): 1 not enough free pages, 2 a sequence longer than its table row, 4 a
  * sequence, count or position out of range, 8 a sequence twice in a call or a fork into one
- * that is not empty, 16 a position past its sequence's end, 32 a table entry that is no page.
+ * that is not empty, 16 a position past its sequence's end (one that an append was refused among
+ * them), 32 a table entry that is no page.
  * Either pointer may be NULL.  Refused while the stream is being captured. */
 int    coli_hip_pages_status(const ColiHipPages *p, int *n_free, int *errors, void *stream);
 
@@ -381,11 +384,12 @@ typedef struct {
 } ColiHipHeads;
 int    coli_hip_heads_check(const ColiHipPages *p, const ColiHipHeads *h);
 /* Rows i < n of q, k and v of sequence d_seq[i] at position d_pos[i] (d_pos NULL: the last one,
- * lens - 1): queries normed and rotated into d_qout [n][H][hd], keys normed, rotated and rounded
- * into the sequence's page of the layer, values rounded beside them.  The position must be held
- * already (append first): a row past the end, or with sequence -1, is skipped whole.  Two rows
- * with one position leave either's K and V.  Angles are pos * freq in 64 bits.  d_qout overlaps no
- * input. */
+ * lens - 1, which the append before gave it): queries normed and rotated into d_qout [n][H][hd],
+ * keys normed, rotated and rounded into the sequence's page of the layer, values rounded beside
+ * them.  The position must be held already (append first): a row past the end, with sequence -1, or
+ * (d_pos NULL) of a sequence that was refused its place is skipped whole, its row of d_qout left as
+ * it was; so is, with no error bit, a row of position -1 or of an empty sequence.  Two rows with one
+ * position leave either's K and V.  Angles are pos * freq in 64 bits.  d_qout overlaps no input. */
 int    coli_hip_qk_rope_paged(const ColiHipPages *p, const ColiHipHeads *h, int layer, const float *d_q,
                               const float *d_k, const float *d_v, const int *d_seq, const int *d_pos, int n,
                               float *d_qout, void *stream);
@@ -405,7 +409,7 @@ int    coli_hip_attn_paged(const ColiHipPages *p, const ColiHipHeads *h, int lay
 /* An attention layer of n rows of many sequences, the batch form of coli_vk_gqa_full on device
  * rows: d_x [n][D] (normed) -> q (| gate where gq_t has 2 H hd rows), k, v -> qk_rope into the
  * pages -> attention -> out_t -> d_out [n][out_t rows].  The positions must have been appended.
- * A row with sequence -1, or past its sequence's end, gives 0.  The strides of h are not used.  Shares the layer blocks'
+ * A row that qk_rope skips gives 0.  The strides of h are not used.  Shares the layer blocks'
  * scratch: one stream, and not one that is being captured. */
 int    coli_hip_gqa_paged(const ColiHipPages *p, const ColiHipHeads *h, int layer, const float *d_x, int D,
                           const ColiVkTensor *gq_t, const ColiVkTensor *gk_t, const ColiVkTensor *gv_t,

@@ -38,7 +38,16 @@ struct HeadsView {
     const float *qn, *kn, *freq;
 };
 
-// The last position that row n sees (-1: none), and its sequence (-1: no row).
+// Scratch of `work` in ints; behind it a word per sequence.  The word is refused_at(len) after a call that
+// was to grow the sequence at that length and was refused; no other call leaves that value for a length it
+// gives the sequence.
+constexpr size_t work_ints(int n_pages) { return 2 * (size_t)n_pages + 64; }
+__device__ __forceinline__ int refused_at(int len) { return len ^ (int)0xA5C35A3Cu; }
+__device__ __forceinline__ int &grow_word(const PoolView &p, int s) { return p.work[work_ints(p.n_pages) + s]; }
+
+// The last position that row n sees (-1: none), and its sequence (-1: no row).  kNew: the row brings that
+// position's keys and values; without pos it has none (-2) when its sequence was refused the place for it.
+template <bool kNew = false>
 __device__ __forceinline__ int row_pos(const PoolView &p, const int *seq, const int *pos, int n, int &s) {
     s = seq[n];
     if (s < 0 || s >= p.n_seqs) {
@@ -46,7 +55,12 @@ __device__ __forceinline__ int row_pos(const PoolView &p, const int *seq, const 
         s = -1;
         return -1;
     }
+    const int word = kNew && !pos ? grow_word(p, s) : 0;
     const int len = min(max(p.lens[s], 0), p.max_pages * p.page), at = pos ? pos[n] : len - 1;
+    if (kNew && !pos && word == refused_at(len)) {
+        atomicOr(&p.state[kStErr], kPgPos);
+        return -2;
+    }
     if (at < len && at >= -1) return at;
     atomicOr(&p.state[kStErr], at < -1 ? kPgIndex : kPgPos);
     return at < -1 ? -2 : -3 - len;   // -2: no position; -3 - len: past the end

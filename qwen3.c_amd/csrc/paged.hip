@@ -95,7 +95,7 @@ __global__ __launch_bounds__(64 * kRopeWaves) void qk_rope_rows(PoolView p, Head
 #pragma unroll
     for (int i = 0; i < 2; i++) fr[i] = lane + 64 * i < hr ? h.freq[lane + 64 * i] : 0.f;
     int s;
-    const int at = row_pos(p, seq, pos, n, s);
+    const int at = row_pos<true>(p, seq, pos, n, s);
     if (s < 0 || at < 0) return;
     const int pj = at / p.page, slot = at - pj * p.page;
     const int pg = p.table[(size_t)s * p.max_pages + pj];
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(256) void block_rows(PoolView p, const int *__restr
     if (i < nc) ctx[i] = 0.f;
     if (i < (size_t)n) {
         int s;
-        live[i] = row_pos(p, seq, pos, (int)i, s) < 0 ? -1 : s;
+        live[i] = row_pos<true>(p, seq, pos, (int)i, s) < 0 ? -1 : s;
     }
 }
 

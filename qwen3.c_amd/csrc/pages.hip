@@ -7,7 +7,8 @@
 // depends on the order of atomics: pages are taken lowest free one first in the order of the
 // call, counts are integers, and a page's bit falls with the count that reaches 0.  A page that
 // is not full belongs to one sequence alone (fork copies it), so a new position never lands in
-// a shared page.
+// a shared page; a step whose append was refused has no position to write, and the sequences'
+// words (paged.h) tell the rotation so.
 //
 // The copies are bound by their bytes: 20 of 40 sequences replaced with the pool closed up, 530 MB
 // moved, 227 us for the four launches (the move 197 us, 5.4 TB/s); six sequences copied whole, 209 MB,
@@ -197,6 +198,10 @@ __global__ __launch_bounds__(T) void pages_take(PoolView p, const int *__restric
     }
     if (!err && total > (long)found + rest) err = kPgFull;
     if (err) {
+        if (mode == kTakeAppend)
+#pragma unroll
+            for (int k = 0; k < kTakeN; k++)
+                if (s[k] >= 0 && (!count || count[tid * kTakeN + k])) grow_word(p, s[k]) = refused_at(p.lens[s[k]]);
         if (tid == 0) {
             atomicOr(&p.state[kStErr], err);
             p.state[kStGo] = 0;
@@ -209,7 +214,9 @@ __global__ __launch_bounds__(T) void pages_take(PoolView p, const int *__restric
         const int i = tid * kTakeN + k;
         if (i < n) s_off[i] = (int)off, s_first[i] = first[k];
         off += need[k];
-        if (s[k] >= 0) p.lens[s[k]] = grown[k];
+        if (s[k] < 0) continue;
+        p.lens[s[k]] = grown[k];
+        if (mode != kTakeAppend || !count || count[i]) grow_word(p, s[k]) = 0;
     }
     if (tid == 0) s_off[n] = (int)total, p.state[kStGo] = 1;
     // the lowest `total` free pages, in order, into the list
@@ -335,7 +342,10 @@ __global__ __launch_bounds__(kCopyThreads) void pages_drop(PoolView p, const int
         return;
     }
     int *row = p.table + (size_t)s * p.max_pages, next = -1;
-    if (threadIdx.x == 0) s_len = atomicExch(&p.lens[s], 0);
+    if (threadIdx.x == 0) {
+        s_len = atomicExch(&p.lens[s], 0);
+        grow_word(p, s) = 0;
+    }
     if (threadIdx.x < p.max_pages) next = row[threadIdx.x];
     __syncthreads();
     const int np = min(pages_of(s_len, p.page), p.max_pages);
@@ -426,7 +436,7 @@ __global__ __launch_bounds__(kCopyThreads) void pages_move(PoolView p, int piece
 __global__ __launch_bounds__(256) void pages_clear(PoolView p) {
     const size_t i0 = blockIdx.x * 256 + threadIdx.x, step = (size_t)gridDim.x * 256;
     for (size_t i = i0; i < (size_t)p.n_seqs * p.max_pages; i += step) p.table[i] = -1;
-    for (size_t i = i0; i < (size_t)p.n_seqs; i += step) p.lens[i] = 0;
+    for (size_t i = i0; i < (size_t)p.n_seqs; i += step) p.lens[i] = grow_word(p, (int)i) = 0;
     for (size_t i = i0; i < (size_t)p.n_pages; i += step) p.refs[i] = 0;
     for (size_t i = i0; i < (size_t)(p.n_pages + 31) / 32; i += step) p.used[i] = 0;
     for (size_t i = i0; i < COLI_HIP_PAGES_STATE; i += step) p.state[i] = 0;
@@ -442,7 +452,7 @@ COLI_API int coli_hip_pages_check(const ColiHipPages *p) {
 }
 
 COLI_API size_t coli_hip_pages_work(const ColiHipPages *p) {
-    return p && p->n_pages > 0 ? 2 * (size_t)p->n_pages + 64 : 0;
+    return p && p->n_pages > 0 ? work_ints(p->n_pages) + (p->n_seqs > 0 ? p->n_seqs : 0) : 0;
 }
 
 COLI_API int coli_hip_pages_init(const ColiHipPages *p, void *stream_) {

@@ -1,0 +1,208 @@
+"""Edges of the paged key-value cache on the GPU: steps that run out of pages, rows over bad pages,
+infinities at odd head dims, calls at once, the largest batches."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import _layers
+import _paged
+import _util
+from _paged import BF16, F16, F32, Pool, addr, ints
+from test_gpu_paged import Attn, sync
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def mod():
+    return _util.load_product()
+
+
+@pytest.fixture(scope="module")
+def dev(torch_dev):
+    return torch_dev
+
+
+# ---------------------------------------------------------------- an append that is refused
+H, KH, HD, PAGE = 4, 2, 16, 4
+
+
+class Step:
+    """A decode step of two layers (append, then rows at their sequences' last positions) over a pool."""
+
+    def __init__(self, mod, lib, dev, pool, n):
+        self.lib, self.dev, self.pool, self.n = lib, dev, pool, n
+        self.att = Attn(mod, lib, dev, pool, H, False)
+        self.heads = mod.Lib.heads(H=H, rot=0, interleaved=0, q_row=H * HD, q_head=HD, kv_row=KH * HD, eps=1e-6,
+                                   rope_mag=1.0, scale=0.25)
+        self.seq = ints([-1] * n, dev)
+        self.x = [torch.zeros(n, h * HD, device=dev) for h in (H, KH, KH)]
+        self.qo, self.out = (torch.zeros(2, n, H, HD, device=dev) for _ in range(2))
+
+    def run(self, st):
+        lib, c, n = self.lib, self.pool.c, self.n
+        lib.pages_append(c, addr(self.seq), None, n, st)
+        for l in range(2):
+            lib.qk_rope_paged_dev(c, self.heads, l, *(addr(t) for t in self.x), addr(self.seq), None, n,
+                                  addr(self.qo[l]), st)
+            lib.attn_paged_dev(c, self.att.heads, l, addr(self.qo[l]), None, addr(self.seq), None, n, 0,
+                               addr(self.out[l]), addr(self.att.work), self.att.work.numel(), st)
+
+    def capture(self):
+        self.run(None)   # of no sequences: the kernels are loaded before the capture
+        sync(self.lib)
+        side, self.graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph, stream=side):
+            self.run(torch.cuda.current_stream().cuda_stream)
+
+    def replay(self, seq, seed):
+        g = torch.Generator().manual_seed(seed)
+        for t in self.x:
+            t.copy_(torch.randn(t.shape, generator=g))
+        self.seq.copy_(ints(seq, self.dev))
+        self.qo.fill_(5.0)
+        torch.cuda.synchronize()
+        self.graph.replay()
+        torch.cuda.synchronize()
+        return self.lib.pages_status(self.pool.c)
+
+
+def written(pool, step, data, seq, lens):
+    """`data` with the rows of the step at the last positions of its sequences."""
+    for r, s in enumerate(seq):
+        if s >= 0:
+            at = lens[s] - 1
+            pg = int(pool.table[s, at // PAGE])
+            for kv in (0, 1):
+                data[pg, :, kv, :, at % PAGE] = step.x[1 + kv][r].view(KH, HD).to(data.dtype)
+    return data
+
+
+@pytest.mark.parametrize("why", ["shared", "own", "row"])
+def test_refused_append_writes_nothing(mod, lib, dev, why):
+    """A captured step whose append is refused (no free page, the last page of two branches shared or
+    not; a table row that is full) changes no page, for any sequence of the batch; the same graph goes
+    on once pages are free or the full sequence is out of the batch."""
+    full = why == "row"
+    pool = Pool(mod, lib, dev, F32, 2, KH, HD, PAGE, 20 if full else {"shared": 6, "own": 8}[why], 4,
+                2 if full else 6, seed=3)
+    pool.place([8, 0 if why == "shared" else 6 if full else 8, 0 if full else 12, 0])
+    if why == "shared":
+        lib.pages_fork(pool.c, addr(a := ints([0], dev)), addr(b := ints([1], dev)), 1, True)
+        sync(lib)
+        assert pool.table[0, :2].tolist() == pool.table[1, :2].tolist()
+    step = Step(mod, lib, dev, pool, 3)
+    step.capture()
+    lens, data, table = pool.lens.tolist(), pool.data.clone(), pool.table.clone()
+    for t in range(2):
+        free, err = step.replay([1, -1, 0], t)
+        assert err == (2 if full else 1) | 16 and pool.lens.tolist() == lens
+        assert torch.equal(pool.data, data) and torch.equal(pool.table, table)
+        assert bool((step.qo == 5.0).all())
+    if full:
+        seq = [1, -1, -1]
+    else:
+        seq = [1, -1, 0]
+        lib.pages_free(pool.c, addr(x := ints([2], dev)), 1)
+        sync(lib)
+    for t in range(2, 4):
+        before = pool.data.clone()
+        free, err = step.replay(seq, t)
+        for s in seq:
+            lens[s] += s >= 0
+        if not full:
+            lens[2] = 0
+        assert err == 0 and pool.lens.tolist() == lens
+        assert torch.equal(pool.data, written(pool, step, before, seq, lens)), t
+        for r, s in enumerate(seq):
+            assert torch.equal(step.qo[1, r].view(-1), step.x[0][r] if s >= 0 else torch.full((H * HD,), 5.0, device=dev))
+    n = [lens[s] for s in seq]
+    step.att.check(torch.where(torch.tensor(seq)[:, None, None] < 0, 77.0, step.out[1].cpu()), step.qo[1].cpu(),
+                   torch.zeros(3, step.att.heads.q_row), seq, n, layer=1)
+
+
+def test_refused_append_is_forgotten(mod, lib, dev):
+    """What a refused append leaves holds only until its sequence grows, is freed or forked into, also where
+    the length comes to the same again; a count of 0 asks for no place; an unnamed sequence is not held up."""
+    pool = Pool(mod, lib, dev, F32, 2, KH, HD, PAGE, 9, 6, 6, seed=3)
+    step = Step(mod, lib, dev, pool, 1)
+    keep = []
+
+    def call(f, *lists):
+        t = [ints(v, dev) if isinstance(v, list) else v for v in lists]
+        keep.extend(t)
+        torch.cuda.synchronize()
+        f(pool.c, *(addr(v) if torch.is_tensor(v) else v for v in t))
+
+    def writes(s):
+        """Whether a row without d_pos of sequence s goes to its last position, and the error bits."""
+        before = pool.data.clone()
+        g = torch.Generator().manual_seed(len(keep))
+        for t in step.x:
+            t.copy_(torch.randn(t.shape, generator=g))
+        keep.append(q := ints([s], dev))
+        torch.cuda.synchronize()
+        for l in range(2):
+            lib.qk_rope_paged_dev(pool.c, step.heads, l, *(addr(t) for t in step.x), addr(q), None, 1, addr(step.qo[l]))
+        sync(lib)
+        err = lib.pages_status(pool.c)[1]
+        if torch.equal(pool.data, before):
+            return False, err
+        assert torch.equal(pool.data, written(pool, step, before, [s], pool.lens.tolist()))
+        return True, err
+
+    call(lib.pages_append, [0, 1, 2], [8, 8, 8], 3)             # 6 of 9 pages
+    for s in range(3):
+        assert writes(s) == (True, 0)
+    call(lib.pages_append, [0, 1, 3], [4, 0, 40], 3)            # refused: 0 and 3, the row of 3 too short
+    assert lib.pages_status(pool.c) == (3, 2)
+    assert writes(0) == (False, 16) and writes(1) == (True, 0) and writes(2) == (True, 0) and writes(3) == (False, 16)
+    call(lib.pages_append, [0], [0], 1)                         # grows by nothing: still without its place
+    assert writes(0) == (False, 16)
+    call(lib.pages_free, [0], 1)
+    call(lib.pages_append, [0], [8], 1)                         # the same length again
+    assert writes(0) == (True, 0)
+    call(lib.pages_append, [2, 9], [1, 1], 2)                   # refused for the other's sake
+    assert lib.pages_status(pool.c)[1] == 4
+    assert writes(2) == (False, 16)
+    call(lib.pages_free, [2], 1)
+    call(lib.pages_fork, [0], [2], 1, 1)                        # as long as before, by a fork
+    assert writes(2) == (True, 0)
+    call(lib.pages_append, [1], [-1], 1)
+    assert lib.pages_status(pool.c)[1] == 4 and writes(1) == (False, 16)
+    call(lib.pages_append, [1], [1], 1)
+    assert writes(1) == (True, 0)
+    call(lib.pages_append, [1, 1], None, 2)
+    assert lib.pages_status(pool.c)[1] == 8 and writes(1) == (False, 16)
+    lib.pages_init(pool.c)
+    call(lib.pages_append, [1], [9], 1)
+    assert writes(1) == (True, 0)
+
+
+def test_refused_append_layer_block(mod, lib, gen, dev):
+    """The layer block of a step without pages gives 0 and keeps the cache."""
+    D, rot, gs = 256, 16, 128
+    W = _layers.GqaWeights(gen, gen.stream(0x9F00, 1), D, 4, 2, 64, rot, gs)
+    tq, tk, tv, to = (m.upload(lib) for m in (W.q, W.k, W.v, W.o))
+    pool = Pool(mod, lib, dev, BF16, 1, 2, 64, 4, 4, 2, 4, seed=2)
+    freq = torch.tensor([float(np.float32(float(W.theta) ** (-2.0 * j / rot))) for j in range(rot // 2)], device=dev)
+    heads = mod.Lib.heads(H=4, rot=rot, interleaved=0, q_row=8 * 64, q_head=2 * 64, kv_row=2 * 64, eps=1e-6,
+                          rope_mag=1.0, scale=1.0 / math.sqrt(64), freq=addr(freq))
+    x = torch.from_numpy(np.concatenate([gen.normal(D, 0x9F10 + t) for t in range(2)])).to(dev)
+    seq, cnt = ints([0, 1], dev), ints([8, 7], dev)
+
+    def go(count):
+        out = torch.full((2, D), 4.0, device=dev)
+        torch.cuda.synchronize()
+        lib.pages_append(pool.c, addr(seq), addr(count), 2)
+        lib.gqa_paged_dev(pool.c, heads, 0, addr(x), tq, tk, tv, to, addr(seq), None, 2, 9, addr(out))
+        sync(lib)
+        return out, lib.pages_status(pool.c)[1]
+
+    out, err = go(cnt)
+    assert err == 0 and bool(out.any(1).all())
+    data = pool.data.clone()
+    out, err = go(None)
+    assert err == 1 | 16 and not bool(out.any()) and torch.equal(pool.data, data)
