@@ -19,9 +19,10 @@
 // weights by 2^kUp).  The pieces are further rows of the same products: GS (4, 8 or 16) rows per
 // piece, so 8 heads in f16 and 4 in bf16 cost one product, and the 16 rows are seldom idle.
 // The f32 products they replace took 8 times the matrix cycles of one 16-bit product.
-//   A piece times an infinity can be NaN where the product is infinite: when a result is not
-// finite, the block computes its part again in plain fp32 (slow_part), which gives what the
-// formula gives.
+//   A piece times an infinity can be NaN where the product is infinite, and so can the zeros that q is
+// padded with to the kernel's head dim (the keys' first columns are loaded again there): when a result
+// is not finite, the block computes its part again in plain fp32 (slow_part), which gives what the
+// formula gives.  Pages of f32 at the kernels' own head dims have no such zeros.
 //
 // Work: a unit is kKeys keys (a tile per wave) of a kv head, 64 KB or so; a (row, kv head) counts
 // kSetup units more, about what its q, row offsets and sums cost beside the keys (200 ragged rows of
@@ -685,8 +686,9 @@ __global__ __launch_bounds__(64 * W, resident(T, HD, W)) void attn_part(PoolView
                 for (int e = 0; e < kVE; e += 4) *(float4 *)(dst + e) = *(const float4 *)(o + e);
             }
         }
-        // the sums' place is the next part's q; 16-bit products that met an infinity or NaN: again
-        if (__syncthreads_or(!kWide && z != 0.f))
+        // the sums' place is the next part's q; products that met an infinity or NaN: again, where pieces or
+        // the zeros of q past the head dim may have made a NaN of what is none
+        if (__syncthreads_or(!(kWide && kExact) && z != 0.f))
             slow_part<T, W>(p, h, a, r, s, kh, head, hn, cnt, from, last, whole, slot, s_o, &s_m[0][0]);
         if (c0 == 0 && !direct) {   // u is behind its unit c1
             cut = Cut{};

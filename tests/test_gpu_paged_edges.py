@@ -206,3 +206,39 @@ def test_refused_append_layer_block(mod, lib, gen, dev):
     data = pool.data.clone()
     out, err = go(None)
     assert err == 1 | 16 and not bool(out.any()) and torch.equal(pool.data, data)
+
+
+# ---------------------------------------------------------------- infinities at head dims of their own
+@pytest.mark.parametrize("hint", [0, 200], ids=["shares", "whole"])
+@pytest.mark.parametrize("hd", [8, 72, 80, 176])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "f16", "f32"])
+def test_attn_minus_infinity(mod, lib, dev, dtype, hd, hint):
+    """A key with -inf in a column where the queries are positive has no weight, whatever the head dim
+    is padded to; +inf there and NaN give NaN, for its heads alone; an infinity of V stays in its column."""
+    KH, page, length = 2, 16, 200
+    pool = Pool(mod, lib, dev, dtype, 1, KH, hd, page, 5 * 13 + 1, 5, 14, seed=4)
+    pool.place([length] * 5)
+    a = Attn(mod, lib, dev, pool, 4, True, seed=3)
+    q, raw = a.rows(5)
+    q[:3, :, :4], q[0, 2:, hd - 1] = q[:3, :, :4].abs(), q[0, 2:, hd - 1].abs()
+    t, inf = pool.table.long(), float("inf")
+    clean = a.run(q, raw, list(range(5)), max_len=hint)
+    a.check(clean, q, raw, list(range(5)), [length] * 5)
+    pool.data[t[0, 3], 0, 0, 0, 5, 0] = -inf         # the first column of the key
+    pool.data[t[0, 12], 0, 0, 0, 2, 3] = -inf
+    pool.data[t[0, 7], 0, 0, 1, 9, hd - 1] = -inf    # the last
+    pool.data[t[1, 0], 0, 0, 1, 0, 1] = inf
+    pool.data[t[2, 1], 0, 0, 0, 1, 2] = float("nan")
+    pool.data[t[3, 2], 0, 1, 1, 3, hd - 2] = inf
+    torch.cuda.synchronize()
+    got = a.run(q, raw, list(range(5)), max_len=hint)
+    K, V = (pool.rows(0, 0, length, i) for i in (0, 1))
+    fin = torch.isfinite(K).all(-1)
+    want = torch.cat([_paged.attn(q[0, 2 * h:2 * h + 2], K[h:h + 1, fin[h]], V[h:h + 1, fin[h]], a.scale,
+                                  a.gate_of(raw, 0)[2 * h:2 * h + 2])[0] for h in range(KH)])
+    assert torch.allclose(got[0].double(), want, rtol=1e-5, atol=1e-5)
+    assert bool(torch.isnan(got[1, 2:]).all()) and bool(torch.isnan(got[2, :2]).all())
+    assert bool((got[3, 2:, hd - 2] == inf).all())
+    rest = clean.clone()
+    rest[0], rest[1, 2:], rest[2, :2], rest[3, 2:, hd - 2] = got[0], got[1, 2:], got[2, :2], got[3, 2:, hd - 2]
+    assert torch.allclose(got, rest, rtol=2e-5, atol=2e-5, equal_nan=True)
