@@ -319,8 +319,8 @@ int   coli_hip_gdn_chunked(int on);
  * (not data).  hd is a multiple of 8 in 8..256, page 1..4096, max_pages * page at most 2^30.
  * The functions read and change the arrays on the device, in stream order, with no host
  * decision: a decode step (append, then per layer qk_rope and attn) can be captured into a
- * graph.  Calls on one pool that change it (init, append, fork, free, compact, qk_rope) must be
- * ordered: one stream, or events between streams.  In every list of sequences -1 stands for
+ * graph.  Calls on one pool that change it (init, append, fork, free, compact, qk_rope, status) must
+ * be ordered: one stream, or events between streams.  In every list of sequences -1 stands for
  * "none" (padding of a fixed-size batch).  What only the device can see is not reported by the
  * return value but gathered in the pool's error bits (coli_hip_pages_status). */
 enum { COLI_HIP_F32 = 0, COLI_HIP_F16 = 1, COLI_HIP_BF16 = 2 };

@@ -16,8 +16,8 @@ enum {
     kPgPage = 32,     // a table entry that is no page
 };
 // Words of the pool's state: the error bits; what a bookkeeping kernel leaves to the copy
-// kernel behind it on the stream (go; pages to move, pages in use).
-enum { kStErr = 0, kStGo = 1, kStMove = 2, kStLive = 3 };
+// kernel behind it on the stream (go; pages to move, pages in use); the error bits that a status call took.
+enum { kStErr = 0, kStGo = 1, kStMove = 2, kStLive = 3, kStSeen = 4 };
 
 // ColiHipPages with its derived strides, by value to every kernel.
 struct PoolView {

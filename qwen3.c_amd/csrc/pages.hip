@@ -442,6 +442,9 @@ __global__ __launch_bounds__(256) void pages_clear(PoolView p) {
     for (size_t i = i0; i < COLI_HIP_PAGES_STATE; i += step) p.state[i] = 0;
 }
 
+// The error bits, taken in one step: attention on another stream may be setting more.
+__global__ void pages_errors(PoolView p) { p.state[kStSeen] = atomicExch(&p.state[kStErr], 0); }
+
 }  // namespace coli
 
 using namespace coli;
@@ -531,12 +534,11 @@ COLI_API int coli_hip_pages_status(const ColiHipPages *p, int *n_free, int *erro
     unsigned *h = (unsigned *)malloc((size_t)words * 4);
     if (!h) return 0;
     int err = 0;
-    const int zero = 0;
-    hipError_t e = hipMemcpyAsync(h, v.used, (size_t)words * 4, hipMemcpyDeviceToHost, st);
-    if (e == hipSuccess) e = hipMemcpyAsync(&err, v.state + kStErr, 4, hipMemcpyDeviceToHost, st);
+    hipLaunchKernelGGL(pages_errors, dim3(1), dim3(1), 0, st, v);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) e = hipMemcpyAsync(h, v.used, (size_t)words * 4, hipMemcpyDeviceToHost, st);
+    if (e == hipSuccess) e = hipMemcpyAsync(&err, v.state + kStSeen, 4, hipMemcpyDeviceToHost, st);
     if (e == hipSuccess) e = hipStreamSynchronize(st);
-    if (e == hipSuccess && err) e = hipMemcpyAsync(v.state + kStErr, &zero, 4, hipMemcpyHostToDevice, st);
-    if (e == hipSuccess && err) e = hipStreamSynchronize(st);
     int fr = 0;
     for (int w = 0; e == hipSuccess && w < words; w++) {
         const int left = v.n_pages - w * 32;

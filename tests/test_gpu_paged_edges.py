@@ -242,3 +242,29 @@ def test_attn_minus_infinity(mod, lib, dev, dtype, hd, hint):
     rest = clean.clone()
     rest[0], rest[1, 2:], rest[2, :2], rest[3, 2:, hd - 2] = got[0], got[1, 2:], got[2, :2], got[3, 2:, hd - 2]
     assert torch.allclose(got, rest, rtol=2e-5, atol=2e-5, equal_nan=True)
+
+
+# ---------------------------------------------------------------- calls at once
+def test_status_loses_no_bits(mod, lib, dev):
+    """Error bits that an attention call on another stream sets while the status is read are in this
+    reading or in the next."""
+    pool = Pool(mod, lib, dev, BF16, 1, 1, 64, 16, 64, 2, 32, seed=4)
+    pool.place([400, 100])
+    a, b = (Attn(mod, lib, dev, pool, 4, False, seed=i) for i in (1, 2))
+    q = a.rows(1)[0].to(dev)
+    out = [torch.zeros(1, 4, 64, device=dev) for _ in range(2)]
+    none, one, far = ints([-2], dev), ints([0], dev), ints([4000], dev)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for t in range(400):
+        lib.attn_paged_dev(pool.c, a.heads, 0, addr(q), None, addr(none), None, 1, 0, addr(out[0]), addr(a.work),
+                           a.work.numel())                                             # bit 4
+        lib.sync()
+        for i in range(t % 20 + 1):   # the last one sets bit 16, later from turn to turn
+            lib.attn_paged_dev(pool.c, b.heads, 0, addr(q), None, addr(one), addr(far) if i == t % 20 else None, 1, 0,
+                               addr(out[1]), addr(b.work), b.work.numel(), side.cuda_stream)
+        first = lib.pages_status(pool.c)[1]
+        torch.cuda.synchronize()
+        second = lib.pages_status(pool.c)[1]
+        assert first | second == 4 | 16, (t, first, second)
+    assert lib.pages_status(pool.c)[1] == 0
