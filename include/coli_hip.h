@@ -395,13 +395,14 @@ int    coli_hip_qk_rope_paged(const ColiHipPages *p, const ColiHipHeads *h, int 
                               float *d_qout, void *stream);
 /* Attention of row i over positions 0..d_pos[i] of sequence d_seq[i] (d_pos NULL: all of it):
  * d_out [n][H][hd] = softmax(scale q k^T) v, times sigmoid(gate) where d_gate is not NULL
- * (strides q_row, q_head).  d_q is [n][H][hd] as qk_rope leaves it.  A row that sees no position
- * gives 0; a row with sequence -1 is left as it was; one past the end sees what the sequence
- * holds.  max_len: the longest sequence in the call as far as the caller knows (0: unknown); only the split
- * of the work goes by it (short rows take one launch instead of two).  Sums of values times weights are held in fp32 before they are divided
- * by the weights' sum: values past 2^88 in magnitude may give infinities.  d_out overlaps no
- * input; d_out and d_work are aligned to 16 bytes;
- * d_work: coli_hip_attn_paged_work() bytes, not shared by calls that may run at once, no contents kept. */
+ * (strides q_row, q_head).  d_q is [n][H][hd] as qk_rope leaves it.  Positions whose table entry is
+ * no page are left out.  A row that sees no position gives 0; a row with sequence -1 is left as it
+ * was; one past the end sees what the sequence holds.  max_len: the longest sequence in the call as
+ * far as the caller knows (0: unknown); only the split of the work goes by it (short rows take one
+ * launch instead of two).  Sums of values times weights are held in fp32 before they are divided by
+ * the weights' sum: values past 2^88 in magnitude may give infinities.  d_out overlaps no input;
+ * d_out and d_work are aligned to 16 bytes; d_work: coli_hip_attn_paged_work() bytes, not shared by
+ * calls that may run at once, no contents kept. */
 size_t coli_hip_attn_paged_work(const ColiHipPages *p, const ColiHipHeads *h);
 int    coli_hip_attn_paged(const ColiHipPages *p, const ColiHipHeads *h, int layer, const float *d_q,
                            const float *d_gate, const int *d_seq, const int *d_pos, int n, int max_len, float *d_out,

@@ -48,6 +48,7 @@ constexpr int kGroup = 16;        // heads a wave takes
 constexpr int kLaneRows = 8;      // rows of a lane while they are lined up: 512 rows or fewer
 constexpr float kLazy = 8.f;      // the maximum moves when a score passes it by 2^8: weights stay below
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoKeys = -1.f;   // the sum of the weights of a part none of whose keys are there (others': 0 or more)
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
@@ -169,13 +170,13 @@ __device__ __forceinline__ float sum_pieces(float x) {
     return x;
 }
 
-// N sums over the weights' sum (a row of no keys: 0), times the gate.  The divisions, each a chain of ten
+// N sums over the weights' sum (a row that has no keys: 0), times the gate.  The divisions, each a chain of ten
 // instructions, and the gate's loads go side by side (one row of 128 keys, gated: 10.7 us one by one, 9.9 so).
 template <int N>
-__device__ __forceinline__ void finish(float *o, float l, int cnt, const float *gate, long at) {
+__device__ __forceinline__ void finish(float *o, float l, int some, const float *gate, long at) {
 #pragma unroll
-    for (int i = 0; i < N; i++) o[i] = cnt ? o[i] / l : 0.f;
-    if (!gate || !cnt) return;
+    for (int i = 0; i < N; i++) o[i] = some ? o[i] / l : 0.f;
+    if (!gate || !some) return;
     float w[N];
 #pragma unroll
     for (int i = 0; i < N; i++) w[i] = gate[at + i];
@@ -184,15 +185,16 @@ __device__ __forceinline__ void finish(float *o, float l, int cnt, const float *
 }
 
 // A part in plain fp32: keys [from, last) of the row, a key per wave at a time, four columns a
-// lane, head by head.
+// lane, head by head.  Where no page of it is one, the row or part is empty: 0, or a sum of -1 for the join.
 template <int T, int W>
 __device__ void slow_part(const PoolView &p, const HeadsView &h, const PagedArgs &a, int r, int s, int kh, long head,
-                          int hn, int cnt, int from, int last, bool whole, long slot, float *s_o, float *s_ml) {
+                          int hn, int from, int last, bool whole, long slot, float *s_o, float *s_ml) {
     constexpr int kUp = Pieces<T>::up, kWaves = W;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = 4 * lane;
     const bool in = d0 < p.hd;
     const int *row = p.table + (size_t)s * p.max_pages;
     const char *base = p.data + (size_t)a.layer * p.layer_bytes + (size_t)kh * p.head_bytes;
+    int seen = 0;
     for (int hh = 0; hh < hn; hh++) {
         float x[4] = {}, o[4] = {}, m = -INFINITY, l = 0.f;
         if (in)
@@ -201,6 +203,7 @@ __device__ void slow_part(const PoolView &p, const HeadsView &h, const PagedArgs
             const unsigned j = page_of(a, t);
             const int pg = row[j];
             if (pg < 0 || pg >= p.n_pages) continue;
+            seen = 1;
             const char *kr = base + (size_t)pg * p.page_bytes + (size_t)(t - j * p.page) * p.row_bytes;
             float k[4] = {}, v[4] = {}, dot = 0.f;
             if (in)
@@ -217,7 +220,7 @@ __device__ void slow_part(const PoolView &p, const HeadsView &h, const PagedArgs
             l = fmaf(l, f, w);
             m = nm;
         }
-        __syncthreads();
+        seen = __syncthreads_or(seen);
         if (in)
             for (int i = 0; i < 4; i++) s_o[wave * 256 + d0 + i] = o[i];
         if (lane == 0) s_ml[2 * wave] = m, s_ml[2 * wave + 1] = l;
@@ -231,10 +234,10 @@ __device__ void slow_part(const PoolView &p, const HeadsView &h, const PagedArgs
         for (int d = threadIdx.x; d < p.hd; d += 64 * W) {
             float t = 0.f;
             for (int w = 0; w < kWaves; w++) t += f[w] * s_o[w * 256 + d];
-            if (whole) finish<1>(&t, L, cnt, a.gate, r * h.q_row + (head + hh) * h.q_head + d);
+            if (whole) finish<1>(&t, L, seen, a.gate, r * h.q_row + (head + hh) * h.q_head + d);
             (whole ? a.out + ((long)r * h.H + head + hh) * p.hd : a.part + (slot * a.stride + hh) * p.hd)[d] = t;
         }
-        if (!whole && threadIdx.x == 0) a.ml[slot * a.stride + hh] = make_float2(M, L);
+        if (!whole && threadIdx.x == 0) a.ml[slot * a.stride + hh] = make_float2(M, seen ? L : kNoKeys);
     }
     __syncthreads();
 }
@@ -644,7 +647,7 @@ __global__ __launch_bounds__(64 * W, resident(T, HD, W)) void attn_part(PoolView
             s_l[wave][c] = l;
         }
         lds_barrier();   // the last loads, of no keys, need not have come
-        float z = 0.f;   // NaN when a result of this thread's is not finite
+        float z = 0.f;   // NaN when a result of this thread's is not finite, 1 when a row's weights are all 0
         {
             float *so = s_o + wave * kSum + 4 * lane;
 #pragma unroll
@@ -674,7 +677,9 @@ __global__ __launch_bounds__(64 * W, resident(T, HD, W)) void attn_part(PoolView
                         for (int w = 0; w < kWaves; w++) o[e] = fmaf(at[w * kSum + 256 * e], f[w], o[e]);
                 }
 #pragma unroll
-                for (int e = 0; e < kVE; e++) z = fmaf(o[e] + L, 0.f, z);
+                for (int e = 0; e < kVE; e++)
+                    if (!(kWide && kExact)) z = fmaf(o[e] + L, 0.f, z);
+                if (L == 0.f && cnt) z += 1.f;
                 float *dst = a.part + (slot * a.stride + hh) * p.hd + d0;
                 if (whole) {
                     dst = a.out + ((long)r * h.H + head + hh) * p.hd + d0;
@@ -687,9 +692,10 @@ __global__ __launch_bounds__(64 * W, resident(T, HD, W)) void attn_part(PoolView
             }
         }
         // the sums' place is the next part's q; products that met an infinity or NaN: again, where pieces or
-        // the zeros of q past the head dim may have made a NaN of what is none
-        if (__syncthreads_or(!(kWide && kExact) && z != 0.f))
-            slow_part<T, W>(p, h, a, r, s, kh, head, hn, cnt, from, last, whole, slot, s_o, &s_m[0][0]);
+        // the zeros of q past the head dim may have made a NaN of what is none.  And where no key had a weight,
+        // to tell scores of -inf (NaN) from pages that are none (0).
+        if (__syncthreads_or(z != 0.f))
+            slow_part<T, W>(p, h, a, r, s, kh, head, hn, from, last, whole, slot, s_o, &s_m[0][0]);
         if (c0 == 0 && !direct) {   // u is behind its unit c1
             cut = Cut{};
             if (c1 < nc) {
@@ -744,6 +750,8 @@ __global__ __launch_bounds__(kJoin) void attn_join(PoolView p, HeadsView h, Page
     if (lane == 0) s_red[wave] = l;
     __syncthreads();
     l = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
+    const bool some = m != -INFINITY || l != n * kNoKeys;   // parts of no keys count with any other part's 0 at most
+    if (m == -INFINITY) l = 0.f;                            // every score is -inf
 #pragma unroll
     for (int j = 0; j < kAhead; j++) {
         const int k = k0 + j * ks;
@@ -762,7 +770,7 @@ __global__ __launch_bounds__(kJoin) void attn_join(PoolView p, HeadsView h, Page
     if (k0 || !in) return;
     for (int k = 1; k < ks; k++) o += s_o[tid + k * wide];
     float y[4] = {o[0], o[1], o[2], o[3]};
-    finish<4>(y, l, 1, a.gate, cut.row * h.q_row + (cut.head + hh) * h.q_head + d);
+    finish<4>(y, l, some, a.gate, cut.row * h.q_row + (cut.head + hh) * h.q_head + d);
     o = v4f{y[0], y[1], y[2], y[3]};
     *(v4f *)(a.out + ((long)cut.row * h.H + cut.head + hh) * p.hd + d) = o;
 }

@@ -268,3 +268,40 @@ def test_status_loses_no_bits(mod, lib, dev):
         second = lib.pages_status(pool.c)[1]
         assert first | second == 4 | 16, (t, first, second)
     assert lib.pages_status(pool.c)[1] == 0
+
+
+# ---------------------------------------------------------------- rows over pages that are none
+@pytest.mark.parametrize("hint", [0, 150, 40], ids=["shares", "whole", "whole-short"])
+@pytest.mark.parametrize("hd", [64, 80])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "f16", "f32"])
+def test_attn_all_pages_bad(mod, lib, dev, dtype, hd, hint):
+    """A row all of whose table entries are no pages sees nothing and gives 0, a short one and one in
+    parts; rows whose first or last keys alone are there see those; a row all of whose keys have -inf
+    scores has no softmax (NaN), as the formula has it, also where its other pages are bad."""
+    KH, page = 2, 16
+    lens = [5, 3000, 40, 3000, 3000, 16, 3000, 3000]
+    pool = Pool(mod, lib, dev, dtype, 1, KH, hd, page, 5 * 188 + 10, 8, 190, seed=4)
+    pool.place(lens)
+    a = Attn(mod, lib, dev, pool, 4, True, seed=3)
+    q, raw = a.rows(8)
+    q[5:7, :, 1] = q[5:7, :, 1].abs() + 0.1
+    t = pool.table
+    t[0, 0] = -1
+    t[1, :188] = pool.n_pages
+    t[2, 0], t[2, 2] = -5, 2 ** 31 - 1               # the middle page alone
+    t[3, :100] = -1                                  # parts of no keys before those that have some
+    t[4, 3:188] = -1                                 # and behind them
+    for s, n in ((5, 1), (6, 188)):
+        pool.data[t[s, :n].long(), 0, 0, :, :, 1] = -float("inf")
+    t[6, 20:120] = -1
+    torch.cuda.synchronize()
+    got = a.run(q, raw, list(range(8)), max_len=hint)
+    assert lib.pages_status(pool.c)[1] == 32
+    assert bool((got[:2] == 0.0).all()), got[:2]
+    for s, keys in ((2, range(16, 32)), (3, range(1600, 3000)), (4, range(48))):
+        held = [p for j, p in enumerate(t[s, :-(-lens[s] // page)].tolist()) if 0 <= p < pool.n_pages]
+        x = pool.data[held, 0].cpu().double().permute(1, 2, 0, 3, 4).reshape(2, KH, -1, hd)[:, :, :len(keys)]
+        want = _paged.attn(q[s], x[0], x[1], a.scale, a.gate_of(raw, s))[0]
+        assert torch.allclose(got[s].double(), want, rtol=1e-5, atol=1e-5), s
+    assert bool(torch.isnan(got[5:7]).all())
+    a.check(got[7:], q[7:], raw[7:], [7], [lens[7]])
