@@ -765,7 +765,14 @@ bool gemv(const ColiVkTensor *t, const float *d_x, float *d_y, int S, hipStream_
                              (int *)((unsigned long long *)g_keys + n)};
         return launch_lanes_mode<2>(t, d_x, d_y, st, ta) != 0;
     }
-    if (S >= kGemmMinS && gemm6_ok(t)) return gemm6(&t, &d_y, 1, d_x, S, st);   // c/backend_vulkan.c:282-299
+    if (S >= kGemmMinS && gemm6_ok(t)) {   // c/backend_vulkan.c:282-299
+        const int most = (int)(((1u << 31) - 1) / (3u * t->I));   // rows of a gemm6 call
+        for (int s = 0; s < S; s += most) {
+            float *y = d_y + (size_t)s * t->O;
+            if (!gemm6(&t, &y, 1, d_x + (size_t)s * t->I, S - s < most ? S - s : most, st)) return false;
+        }
+        return true;
+    }
     if (S >= 2 && !want_k && gemm_f01_ok(t, d_x)) return gemm_f01(t, d_x, d_y, S, st);
     if (!launch_rows(t, d_x, d_y, S, st)) return false;
     return want_k ? topk(d_y, t->O, tk->k, tk->idx, tk->val, st) : true;

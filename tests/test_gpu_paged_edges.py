@@ -305,3 +305,24 @@ def test_attn_all_pages_bad(mod, lib, dev, dtype, hd, hint):
         assert torch.allclose(got[s].double(), want, rtol=1e-5, atol=1e-5), s
     assert bool(torch.isnan(got[5:7]).all())
     a.check(got[7:], q[7:], raw[7:], [7], [lens[7]])
+
+
+# ---------------------------------------------------------------- the largest batches
+def test_projection_of_many_rows(lib, gen, dev):
+    """2^20 rows, what a call of the paged cache may have, through a projection of 1024 columns: rows at
+    both ends and about every border of its pieces against a small call's.  The two may sum in another
+    order: 1024 products of 24 bits, 6 sqrt(1024) half steps of the largest output."""
+    I, O, S = 1024, 48, 1 << 20
+    q, sz = gen.fmt6(O, I, 128, 0xA100)
+    t = lib.tensor(q, sz, 6, I, O, 128)
+    x = torch.randn(S, I, device=dev)
+    most = (2 ** 31 - 1) // (3 * I)
+    rows = [0, 1, 2 ** 18 - 1, 2 ** 18, 2 ** 19, most - 1, most, most + 1, S - 2, S - 1]
+    few = x[rows].contiguous()
+    y, z = torch.full((S, O), float("nan"), device=dev), torch.zeros(len(rows), O, device=dev)
+    torch.cuda.synchronize()
+    lib.gemv_dev(t, addr(x), addr(y), S)
+    lib.gemv_dev(t, addr(few), addr(z), len(rows))
+    lib.sync()
+    assert not bool(torch.isnan(y).any())
+    assert bool(((y[rows] - z).abs() <= 2 * 6 * 32 * _paged.U * z.abs().max()).all())
