@@ -213,9 +213,9 @@ void paged_shutdown() {
 // that the rotation has written their query; others get sequence -1 and keep the zeros.
 __global__ __launch_bounds__(256) void block_rows(PoolView p, const int *__restrict__ seq, const int *__restrict__ pos,
                                                   int n, int *__restrict__ live, float *__restrict__ ctx, size_t nc) {
-    const size_t i = blockIdx.x * (size_t)256 + threadIdx.x;
-    if (i < nc) ctx[i] = 0.f;
-    if (i < (size_t)n) {
+    const size_t i0 = blockIdx.x * (size_t)256 + threadIdx.x, step = gridDim.x * (size_t)256;
+    for (size_t i = i0; i < nc; i += step) ctx[i] = 0.f;
+    for (size_t i = i0; i < (size_t)n; i += step) {
         int s;
         live[i] = row_pos<true>(p, seq, pos, (int)i, s) < 0 ? -1 : s;
     }
@@ -297,10 +297,11 @@ COLI_API int coli_hip_gqa_paged(const ColiHipPages *p, const ColiHipHeads *h, in
     float *qn = (float *)g_pw[P_QN].p, *ctx = (float *)g_pw[P_CTX].p;
     if (!gemv(gq_t, d_x, q, n, st) || !gemv(gk_t, d_x, k, n, st) || !gemv(gv_t, d_x, v, n, st)) return 0;
     int *live = (int *)g_pw[P_SEQ].p;
-    const size_t nc = rows * h->H * hd;   // more than the rows
-    hipLaunchKernelGGL(block_rows, dim3((unsigned)((nc + 255) / 256)), dim3(256), 0, st, pv, d_seq, d_pos, n, live, ctx,
-                       nc);
-    if (!rope_launch(pv, hv, p->dtype, layer, q, k, v, d_seq, d_pos, n, qn, st) ||
+    const size_t nc = rows * h->H * hd, nb = (nc + 255) / 256;   // more than the rows
+    hipLaunchKernelGGL(block_rows, dim3((unsigned)(nb < 65536 ? nb : 65536)), dim3(256), 0, st, pv, d_seq, d_pos, n, live,
+                       ctx, nc);
+    if (!paged_launched("paged layer rows") ||
+        !rope_launch(pv, hv, p->dtype, layer, q, k, v, d_seq, d_pos, n, qn, st) ||
         !attn_paged(pv, hv, p->dtype, layer, qn, gated ? q + hd : nullptr, live, d_pos, n, max_len, ctx,
                      g_pw[P_WORK].p, st))
         return 0;

@@ -326,3 +326,35 @@ def test_projection_of_many_rows(lib, gen, dev):
     lib.sync()
     assert not bool(torch.isnan(y).any())
     assert bool(((y[rows] - z).abs() <= 2 * 6 * 32 * _paged.U * z.abs().max()).all())
+
+
+def test_layer_block_of_many_rows(mod, lib, gen, dev):
+    """A layer block of 2^20 rows, 2^32 values of context: the few rows that have a position, from the
+    first to the last, come out as in a call of their own (the projections' sums in another order), the
+    others give 0."""
+    D, nh, hd, n = 128, 16, 256, 1 << 20
+    tq, tk, tv, to = (lib.tensor(*gen.fmt6(O, I, 128, 0xA200 + i), 6, I, O, 128)
+                      for i, (O, I) in enumerate(((nh * hd, D), (hd, D), (hd, D), (64, nh * hd))))
+    pool = Pool(mod, lib, dev, F32, 1, 1, hd, 4, 12, 3, 4, seed=2)
+    pool.place([13, 9, 16])
+    heads = mod.Lib.heads(H=nh, rot=0, interleaved=0, q_row=nh * hd, q_head=hd, kv_row=hd, eps=1e-6, rope_mag=1.0,
+                          scale=1.0 / math.sqrt(hd))
+    rows = [0, 3, 4095, n // 2, n - 2, n - 1]
+    few_seq, few_pos = ints([0, 1, 2, 0, 1, 2], dev), ints([12, 3, 15, 5, 8, 0], dev)
+    seq, pos = torch.full((n,), -1, dtype=torch.int32, device=dev), torch.zeros(n, dtype=torch.int32, device=dev)
+    seq[rows], pos[rows] = few_seq, few_pos
+    x = torch.randn(n, D, device=dev)
+    few = x[rows].contiguous()
+    out, want = torch.full((n, 64), 3.0, device=dev), torch.full((6, 64), 3.0, device=dev)
+    for hint in (0, 16):
+        out.fill_(3.0)
+        torch.cuda.synchronize()
+        lib.gqa_paged_dev(pool.c, heads, 0, addr(x), tq, tk, tv, to, addr(seq), addr(pos), n, hint, addr(out))
+        sync(lib)
+        lib.gqa_paged_dev(pool.c, heads, 0, addr(few), tq, tk, tv, to, addr(few_seq), addr(few_pos), 6, hint, addr(want))
+        sync(lib)
+        assert lib.pages_status(pool.c)[1] == 0
+        for r in range(6):
+            assert _util.maxrel_scaled(out[rows[r]].cpu().numpy(), want[r].cpu().numpy()) <= 1e-3, r
+        out[rows] = 0.0
+        assert not bool(out.any())
