@@ -404,10 +404,16 @@ def _handles(st):
     return _library(), st["pool"], st.get("heads")
 
 
+def _stream():
+    """torch's current stream, on which the inputs were made and the outputs are read; its default one by
+    the name that is not NULL (the library's own stream): hipStreamLegacy."""
+    return torch.cuda.current_stream().cuda_stream or 1
+
+
 def _own_rope(st):
     lib, pool, heads = _handles(st)
     lib.qk_rope_paged_dev(pool, heads, st["layer"], st["qraw"].data_ptr(), st["kraw"].data_ptr(), st["vraw"].data_ptr(),
-                          st["seq"].data_ptr(), st["pos"].data_ptr(), st["seq"].numel(), st["q"].data_ptr())
+                          st["seq"].data_ptr(), st["pos"].data_ptr(), st["seq"].numel(), st["q"].data_ptr(), _stream())
     return {"q": st["q"], "data": st["data"]}
 
 
@@ -416,15 +422,15 @@ def _own_attn(st):
     c = st["case"]
     gate = st["qraw"].data_ptr() + 4 * c["hd"] if c["gated"] else None
     lib.attn_paged_dev(pool, heads, st["layer"], st["q"].data_ptr(), gate, st["seq"].data_ptr(), None, c["n"],
-                       st["max_len"], st["out"].data_ptr(), st["scratch"].data_ptr(), st["scratch"].numel())
+                       st["max_len"], st["out"].data_ptr(), st["scratch"].data_ptr(), st["scratch"].numel(), _stream())
     return {"out": st["out"]}
 
 
 def _own_fork(st):
     lib, pool, _ = _handles(st)
-    n = st["dst"].numel()
-    lib.pages_free(pool, st["dst"].data_ptr(), n)
-    lib.pages_fork(pool, st["src"].data_ptr(), st["dst"].data_ptr(), n, st["case"]["share"])
+    n, stream = st["dst"].numel(), _stream()
+    lib.pages_free(pool, st["dst"].data_ptr(), n, stream)
+    lib.pages_fork(pool, st["src"].data_ptr(), st["dst"].data_ptr(), n, st["case"]["share"], stream)
     return {k: st[k] for k in ("table", "lens", "refs", "data")}
 
 
@@ -432,9 +438,10 @@ def _own_churn(st):
     lib, pool, _ = _handles(st)
     seq, count, _ = st["groups"][st["turn"]]
     st["turn"] ^= 1
-    lib.pages_free(pool, seq.data_ptr(), seq.numel())
-    lib.pages_compact(pool)
-    lib.pages_append(pool, seq.data_ptr(), count.data_ptr(), seq.numel())
+    stream = _stream()
+    lib.pages_free(pool, seq.data_ptr(), seq.numel(), stream)
+    lib.pages_compact(pool, stream)
+    lib.pages_append(pool, seq.data_ptr(), count.data_ptr(), seq.numel(), stream)
     return {k: st[k] for k in ("table", "lens", "refs", "data")}
 
 
