@@ -28,6 +28,9 @@
  *
  * Plain pointers and sizes only.  `void *stream` is a hipStream_t (NULL = the
  * library's own stream); work issued on it is stream-ordered and not synchronised.
+ * The library's stream is ordered with no other one, the default stream included
+ * (which hipStreamLegacy names here): a program that makes its inputs or reads its
+ * outputs elsewhere passes its stream, or puts events or waits in between.
  */
 #ifndef COLI_HIP_H
 #define COLI_HIP_H

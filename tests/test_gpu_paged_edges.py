@@ -1,6 +1,8 @@
 """Edges of the paged key-value cache on the GPU: steps that run out of pages, rows over bad pages,
 infinities at odd head dims, calls at once, the largest batches."""
+import importlib.util
 import math
+import os
 
 import numpy as np
 import pytest
@@ -358,3 +360,42 @@ def test_layer_block_of_many_rows(mod, lib, gen, dev):
             assert _util.maxrel_scaled(out[rows[r]].cpu().numpy(), want[r].cpu().numpy()) <= 1e-3, r
         out[rows] = 0.0
         assert not bool(out.any())
+
+
+# ---------------------------------------------------------------- calls in a program's stream order
+def _operators():
+    spec = importlib.util.spec_from_file_location("operators", os.path.join(_util.ROOT, "perf", "operators.py"))
+    ops = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ops)
+    return ops
+
+
+@pytest.mark.parametrize("side", [False, True], ids=["default", "side"])
+def test_calls_follow_the_current_stream(dev, side):
+    """Inputs made on torch's current stream, the library's calls, outputs copied on that stream, with no
+    wait between them: as with every step waited for.  Work that takes a while goes ahead of the inputs."""
+    ops, case = _operators(), dict(name="", op="attn", n=16, len=900, ragged=True, H=8, KH=2, hd=64, rot=64, style="half",
+                                   dtype="bf16", page=16, layers=1, gated=True)
+    ops.own = True
+    big = torch.randn(4096, 4096, device=dev)
+    st, other = ops.prepare(case, 1), ops.prepare(case, 2)
+    torch.cuda.synchronize()
+    want, late = (ops.run(s)["out"].clone() for s in (st, other))
+    torch.cuda.synchronize()
+    ops._library().sync()
+    want, late = ops.run(st)["out"].cpu(), ops.run(other)["out"].cpu()
+    q1, q2 = st["q"].clone(), other["q"].clone()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream() if side else torch.cuda.current_stream()):
+        for i in range(6):
+            for s, q in ((st, q1), (other, q2)):
+                s["q"].zero_()
+                s["out"].fill_(-3.0)
+            for _ in range(4):
+                torch.mm(big, big)
+            st["q"].copy_(q1)
+            other["q"].copy_(q2)
+            a = ops.run(st)["out"].clone()
+            b = ops.run(other)["out"].clone()
+            st["out"].fill_(9.0)
+            assert torch.equal(a.cpu(), want) and torch.equal(b.cpu(), late), i
