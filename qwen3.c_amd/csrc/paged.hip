@@ -6,9 +6,6 @@
 #include <math.h>
 #include <stdio.h>
 
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
-
 namespace coli {
 
 static bool heads_view(const ColiHipPages *p, const ColiHipHeads *h, HeadsView &v) {
@@ -33,19 +30,16 @@ struct Val;
 template <>
 struct Val<COLI_HIP_F32> {
     using type = float;
-    static __device__ __forceinline__ float up(float x) { return x; }
     static __device__ __forceinline__ float down(float x) { return x; }
 };
 template <>
 struct Val<COLI_HIP_F16> {
     using type = _Float16;
-    static __device__ __forceinline__ float up(_Float16 x) { return (float)x; }
     static __device__ __forceinline__ _Float16 down(float x) { return (_Float16)x; }
 };
 template <>
 struct Val<COLI_HIP_BF16> {
     using type = __bf16;
-    static __device__ __forceinline__ float up(__bf16 x) { return (float)x; }
     static __device__ __forceinline__ __bf16 down(float x) { return (__bf16)x; }   // to nearest, ties to even
 };
 

@@ -44,6 +44,7 @@
 
 namespace coli {
 
+constexpr int kCUs = 256;         // of a whole card
 constexpr int kGroup = 16;        // heads a wave takes
 constexpr int kLaneRows = 8;      // rows of a lane while they are lined up: 512 rows or fewer
 constexpr float kLazy = 8.f;      // the maximum moves when a score passes it by 2^8: weights stay below
@@ -712,7 +713,7 @@ __global__ __launch_bounds__(64 * W, resident(T, HD, W)) void attn_part(PoolView
 // Block (i, hh, z): columns z * cols.. of head hh of cut i.  A thread has four columns of every
 // ks-th part; the first kAhead parts are on their way while the weights are found.
 constexpr int kAhead = 8, kJoin = 256;
-constexpr int kJoinW = 1024;   // parts whose weights are kept; of more they are taken again
+constexpr int kJoinW = kCUs * 4;   // parts whose weights are kept: a launch's blocks (max_blocks) at most
 __global__ __launch_bounds__(kJoin) void attn_join(PoolView p, HeadsView h, PagedArgs a, int cols) {
     __shared__ float s_w[kJoinW], s_red[kJoin / 64];
     __shared__ v4f s_o[kJoin];
@@ -742,7 +743,7 @@ __global__ __launch_bounds__(kJoin) void attn_join(PoolView p, HeadsView h, Page
     for (int k = tid; k < n; k += kJoin) {
         const float2 ml = a.ml[at(k)];
         const float f = ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
-        if (k < kJoinW) s_w[k] = f;
+        s_w[k] = f;
         l += f * ml.y;
     }
 #pragma unroll
@@ -759,11 +760,7 @@ __global__ __launch_bounds__(kJoin) void attn_join(PoolView p, HeadsView h, Page
     }
     if (in) {
 #pragma unroll 8
-        for (int k = k0 + kAhead * ks; k < min(n, kJoinW); k += ks) o += s_w[k] * *(const v4f *)(a.part + at(k) * p.hd + d);
-        for (int k = kJoinW + k0; k < n; k += ks) {
-            const float x = a.ml[at(k)].x, f = x == m ? 1.f : __builtin_amdgcn_exp2f(x - m);
-            o += f * *(const v4f *)(a.part + at(k) * p.hd + d);
-        }
+        for (int k = k0 + kAhead * ks; k < n; k += ks) o += s_w[k] * *(const v4f *)(a.part + at(k) * p.hd + d);
     }
     s_o[tid] = o;
     __syncthreads();
@@ -775,8 +772,11 @@ __global__ __launch_bounds__(kJoin) void attn_join(PoolView p, HeadsView h, Page
     *(v4f *)(a.out + ((long)cut.row * h.H + cut.head + hh) * p.hd + d) = o;
 }
 
-// Blocks of a launch: all of them resident, so that equal shares end together.
-static int max_blocks(int T, int HD) { return 256 * resident(T, HD); }
+// Blocks of a launch: on a card's 256 CUs all of them are resident, so that equal shares end together (on a
+// partition of fewer CUs they take their turns).  A constant: the workspace's size is asked for without a device.
+static int max_blocks(int T, int HD) { return kCUs * resident(T, HD); }
+static_assert(kJoinW >= kCUs * resident(COLI_HIP_F32, 64) && kJoinW >= kCUs * resident(COLI_HIP_F16, 64),
+              "the join keeps a weight for every block of a launch");
 static int head_dim(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
 // Waves of the blocks where each has a (row, kv head) to itself, or 0: units in equal shares.  us with
