@@ -53,7 +53,7 @@ struct Val<COLI_HIP_BF16> {
 // LP lanes of four columns each, so a wave has 64 / LP rows (query heads, then key heads, then
 // values) at a time and takes more of the same token: the sines and cosines (one pair a lane) and its columns' norm weights
 // are found once.  4005 rows of 32 + 8 heads of 128, all columns turned, f16 pages: 39 us,
-// 4.6 TB/s; a wave per row with its own sines took 111.  192 rows of 16 + 2 heads of 256: 5.3 us.
+// 4.6 TB/s; a wave per row with its own sines took 111.  192 rows of 16 + 2 heads of 256: 6 us.
 constexpr int kRopeWaves = 4;
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v4u4 __attribute__((ext_vector_type(4), aligned(4)));   // rows need not be aligned

@@ -33,8 +33,8 @@
 // no lining up, no second launch.
 //
 // Bound by the bytes of K and V where there are many: two rows of 120000 keys (2 kv heads of 256,
-// f16) 97 us, 5.1 TB/s (a large copy here moves 4.9); 48 rows of up to 16000 keys 68 us, 4.4; the 200
-// rows above 121 us, 4.7.  Bound by a chain of latencies where there are few: one row of 600 keys
+// f16) 97 us, 5.1 TB/s (a large copy here moves 4.9, the library's GEMV reads 6.2); 48 rows of up to 16000
+// keys 68 us, 4.4; the 200 rows above 121 us, 4.7.  Bound by a chain of latencies where there are few: one row of 600 keys
 // 15 us, of which 4 are the join; one of 8 keys, whole, 8.4.  Tried and left out: 32-key tiles for
 // heads of 256 (spills: 48 rows 121 us against 78), more blocks per CU for heads of 128 (154 us with two,
 // 165 with three), blocks of eight waves for whole rows (one row of 600 keys 19.8 us with four, 21.5).
@@ -66,9 +66,10 @@ struct Cut {
     int block, slot;               // of its first part
 };
 
-// Keys of a wave's tile, and waves that fit a SIMD by their registers.  Four for 16-bit heads of 64 spill: 32
-// ragged rows of 2400 keys, 8 kv heads, 22.1 us with four, 17.0 with three; blocks of one wave keep four
-// (500 rows of 32: 11.7 / 12.5).
+// Keys of a wave's tile, and waves of a SIMD (blocks of four waves a CU), which bounds their registers.  Four
+// for 16-bit heads of 64 spill vector registers: 32 ragged rows of 2400 keys, 8 kv heads, 22.1 us with four, 17.0
+// with three.  Blocks of one wave keep four though they spill 7 to 14 (500 rows of 32: 11.7 with four, 12.5 with
+// three; no other shape was measured), and so do f32 pages (2 to 6; three was not measured).
 constexpr int tile_of(int T, int HD) { return T == COLI_HIP_F32 || HD == 256 ? 16 : 32; }
 constexpr int resident(int T, int HD, int W = 4) {
     return HD == 256 ? (T == COLI_HIP_F32 ? 1 : 2) : HD == 128 ? 2 : T == COLI_HIP_F32 || W == 1 ? 4 : 3;
