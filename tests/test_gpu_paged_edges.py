@@ -399,3 +399,35 @@ def test_calls_follow_the_current_stream(dev, side):
             b = ops.run(other)["out"].clone()
             st["out"].fill_(9.0)
             assert torch.equal(a.cpu(), want) and torch.equal(b.cpu(), late), i
+
+
+def test_default_stream_by_its_name(mod, lib, gen, dev):
+    """hipStreamLegacy (1), the name of the default stream that is not NULL: a projection, the layer block,
+    the bookkeeping, the status and the wait, behind torch's work on that stream and ahead of its copies."""
+    D, legacy = 256, 1
+    W = _layers.GqaWeights(gen, gen.stream(0xA300, 1), D, 4, 2, 64, 16, 128)
+    tq, tk, tv, to = (m.upload(lib) for m in (W.q, W.k, W.v, W.o))
+    heads = mod.Lib.heads(H=4, rot=0, interleaved=0, q_row=8 * 64, q_head=2 * 64, kv_row=2 * 64, eps=1e-6,
+                          rope_mag=1.0, scale=0.125)
+    big, xs, lists = torch.randn(4096, 4096, device=dev), torch.randn(5, D, device=dev), ints([0, 1, 2, 3, 4], dev)
+    got = []
+    for stream in (None, legacy):
+        pool = Pool(mod, lib, dev, BF16, 1, 2, 64, 4, 12, 5, 4, seed=2)
+        x, seq, out, y = torch.zeros_like(xs), ints([-1] * 5, dev), torch.zeros(5, D, device=dev), torch.zeros(5, 512, device=dev)
+        torch.cuda.synchronize()
+        for _ in range(8):
+            torch.mm(big, big)
+        x.copy_(xs)
+        seq.copy_(lists)
+        if stream is None:
+            torch.cuda.synchronize()
+        lib.pages_append(pool.c, addr(seq), None, 5, stream)
+        lib.gqa_paged_dev(pool.c, heads, 0, addr(x), tq, tk, tv, to, addr(seq), None, 5, 1, addr(out), stream)
+        lib.gemv_dev(tq, addr(x), addr(y), 5, stream)
+        if stream is None:
+            lib.sync()
+        copies = out.clone(), y.clone(), pool.lens.clone()
+        assert lib.pages_status(pool.c, stream) == (7, 0)
+        lib.sync(stream)
+        got.append(copies)
+    assert bool(got[0][0].any(1).all()) and all(torch.equal(a, b) for a, b in zip(*got))
